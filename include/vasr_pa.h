@@ -70,6 +70,7 @@ typedef enum vasr_pa_status {
 #define VASR_PA_DERR_WAIT_TIMEOUT 0x8  /* a bounded mbarrier wait gave up     */
 #define VASR_PA_DERR_MAPPING_RANGE 0x10 /* copy/swap pair out of range        */
 #define VASR_PA_DERR_QLEN_RANGE 0x20   /* prefill q_len > max_query_len       */
+#define VASR_PA_DERR_POSITION_RANGE 0x40 /* rotary position outside the table  */
 
 int32_t vasr_pa_abi_version(void);
 const char *vasr_pa_status_string(int32_t status);
@@ -441,6 +442,146 @@ int32_t vasr_pa_greedy_argmax(uint32_t *next_ids, const void *logits,
                               const uint8_t *finished, uint32_t *step,
                               void *workspace, size_t workspace_bytes,
                               vasr_pa_stream_t stream);
+
+/*
+ * Rotary embedding with several position axes (time, height, width), as text
+ * mixed with images or video, or a cache whose token places are no longer
+ * positions, needs it (apply_multimodal_rotary_pos_emb at
+ * vasr-models/src/model/thinker_text.rs:1041-1068, with unequal streams).
+ * Frequency i of the R / 2 rotated pairs (i, i + R / 2) takes the position of
+ * one axis, R / 2 = sum of sections[0 .. num_axes):
+ *   interleaved == 0: the first sections[0] frequencies axis 0, the next
+ *     sections[1] axis 1, ...;
+ *   interleaved != 0: with n = num_axes, frequencies a, a + n, a + 2 n, ...
+ *     (sections[a] of them) axis a for every a > 0, all others axis 0.
+ * positions[a * position_axis_stride + t] (int64; a stride of 0 gives every
+ * axis the same positions) indexes cos_table / sin_table, f32
+ * [max_position, R / 2]; a position outside is clamped and sets
+ * VASR_PA_DERR_POSITION_RANGE. Dims R .. head_dim pass unrotated. sections is
+ * a HOST array; num_axes is 1 to 4.
+ *
+ * mrope: x [num_tokens, num_heads, head_dim] with the given token and head
+ * strides (elements; unit dim stride) -> out, strides likewise; out may be x.
+ * inverse != 0 turns by the negative angle, which is also the gradient of the
+ * forward rotation. f32, bf16 or f16; arithmetic in f32, one rounding.
+ */
+int32_t vasr_pa_mrope(void *out, int64_t out_token_stride, int64_t out_head_stride, const void *x,
+                      int64_t x_token_stride, int64_t x_head_stride, const float *cos_table,
+                      const float *sin_table, int64_t max_position, const int64_t *positions,
+                      int64_t position_axis_stride, const int32_t *sections, int32_t num_axes,
+                      int32_t interleaved, int32_t inverse, int64_t num_tokens, int32_t num_heads,
+                      int32_t head_dim, int32_t dtype, vasr_pa_stream_t stream);
+
+/*
+ * The fused pre-attention step with the rotation above: per-head q/k RMSNorm
+ * (both weights NULL: none), rotation of q and k, and the KV append; qkv,
+ * q_out and slot_mapping as for vasr_pa_fused_qk_norm_rope_append. Unlike
+ * that call, nothing is rounded between the norm, the rotation and the store.
+ * cache_dtype is dtype, or VASR_PA_FP8_E4M3 with k_scale / v_scale (device
+ * f32 scalars): k and v are then stored as fp8(value / scale). score_cache
+ * (f32 [num_blocks, num_kv_heads, block_size], may be NULL) is set to 0 at
+ * every appended slot, for vasr_pa_paged_attention_scored. head_dim up to 512.
+ */
+int32_t vasr_pa_fused_qk_norm_mrope_append(
+    void *q_out, const void *qkv, int64_t qkv_token_stride, const void *q_norm_weight,
+    const void *k_norm_weight, float eps, const float *cos_table, const float *sin_table,
+    int64_t max_position, const int64_t *positions, int64_t position_axis_stride,
+    const int32_t *sections, int32_t num_axes, int32_t interleaved, void *key_cache,
+    void *value_cache, float *score_cache, const int64_t *slot_mapping, int64_t num_tokens,
+    int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+    int64_t num_blocks, int32_t dtype, int32_t cache_dtype, const float *k_scale,
+    const float *v_scale, vasr_pa_stream_t stream);
+
+/*
+ * Attention of the last query_len tokens of every sequence over the pages
+ * that also accumulates each cached token's attention weight, the measure by
+ * which vasr_pa_evict_kv keeps tokens. query / out are
+ * [num_seqs * query_len, num_heads, head_dim] (row b * query_len + i; token
+ * stride q_token_stride for query, out contiguous). Row i of sequence b sits
+ * at position context_lens[b] - query_len + i and sees the tokens up to it;
+ * a row before the first token gives zeros. With p the softmax weights,
+ *   score_cache[block(j), h, j % bs] = decay * itself
+ *       + sum over rows i < score_rows and query heads of kv head h of p_j
+ * for every token j < context_lens[b]. score_rows < query_len leaves the
+ * weights of rows out that may not be real yet (drafted tokens). Each query
+ * row's weights are normalised before they are added; scores are f32 and
+ * added in a fixed order. Block tables of different sequences must not name
+ * the same block (it would be scored by both at once), except for the null
+ * block that padding rows share, whose scores mean nothing. f32, bf16 or f16
+ * queries over pages of the same type or fp8; the workspace is scratch that
+ * needs no clearing.
+ */
+size_t vasr_pa_paged_attention_scored_workspace_size(int32_t num_seqs, int32_t query_len,
+                                                     int32_t score_rows, int32_t num_heads,
+                                                     int32_t num_kv_heads, int32_t head_dim,
+                                                     int32_t block_size, int32_t max_context_len);
+int32_t vasr_pa_paged_attention_scored(
+    void *out, const void *query, const void *key_cache, const void *value_cache,
+    float *score_cache, const uint32_t *block_tables, const uint32_t *context_lens,
+    int32_t num_seqs, int32_t query_len, int32_t score_rows, int32_t num_heads,
+    int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int64_t num_blocks,
+    int32_t max_num_blocks_per_seq, int32_t max_context_len, float scale, float softcapping,
+    float decay, int64_t q_token_stride, int32_t dtype, int32_t cache_dtype, const float *k_scale,
+    const float *v_scale, void *workspace, size_t workspace_bytes, vasr_pa_stream_t stream);
+
+/*
+ * Shrink every sequence's cache to at most `budget` tokens. Per kv head the
+ * tokens kept are the first num_sink, the last num_recent (num_sink +
+ * num_recent <= budget) and, of the others, those of the largest score_cache
+ * values; equal scores keep the lower index, NaN is the lowest score. The
+ * kept tokens' K, V and scores move, in their old order, to token places 0,
+ * 1, ... of block_tables (in place: places past the new length keep what
+ * they held), or of out_block_tables [num_seqs, out_max_num_blocks_per_seq]
+ * (may be NULL) whose blocks must be disjoint from block_tables'. A sequence
+ * no longer than its budget keeps everything. budgets (device u32 [num_seqs],
+ * may be NULL) lowers the budget per sequence; where it is under num_sink +
+ * num_recent, the lowest indices of those stay. kept
+ * [num_seqs, num_kv_heads, budget] receives the old indices, ascending, then
+ * -1; new_lens [num_seqs] = min(context_len, budget). In place, block tables
+ * of different sequences must not name the same block. dtype is the pages'
+ * element type (fp8 too).
+ */
+int32_t vasr_pa_evict_kv(void *key_cache, void *value_cache, float *score_cache,
+                         const uint32_t *block_tables, int32_t max_num_blocks_per_seq,
+                         const uint32_t *out_block_tables, int32_t out_max_num_blocks_per_seq,
+                         const uint32_t *context_lens, int32_t max_context_len,
+                         const uint32_t *budgets, int32_t budget, int32_t num_sink,
+                         int32_t num_recent, int32_t *kept, uint32_t *new_lens, int32_t num_seqs,
+                         int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                         int64_t num_blocks, int32_t dtype, vasr_pa_stream_t stream);
+
+/*
+ * Verification of drafted tokens. Row i of target_logits (sequence stride and
+ * row stride in elements, unit column stride, num_drafts + 1 rows) is the
+ * target's answer after the i-th drafted token; p_i = softmax(row i / T) with
+ * T = temperatures[b] (device f32, may be NULL: temperature for all). With
+ * draft_probs (same strides' meaning, f32 / bf16 / f16; NULL: the drafter was
+ * certain, probability 1), draft x_i is accepted while
+ *   uniform[b, i] * q_i(x_i) < p_i(x_i),
+ * and after the n accepted ones the next token is argmax_v r(v) / race[b, v],
+ * r = max(p_n - q_n, 0) where draft n failed (p_n if that is 0 everywhere),
+ * r = p_n after the last draft: with uniform in [0, 1) and race ~ Exp(1) the
+ * tokens are distributed as if sampled from the target alone. T <= 0: drafts
+ * are accepted while they are row i's argmax and the next token is row n's.
+ * Lowest index on ties; NaN logits count as -inf; a row without a logit above
+ * -inf accepts nothing and gives token 0. draft_lens (may be NULL) shortens a
+ * sequence's drafts; draft ids outside the vocabulary are rejected. num_drafts
+ * 0 samples one token. out_tokens [num_seqs, num_drafts + 1]: the accepted
+ * drafts, the next token, then -1; num_accepted [num_seqs]. uniform and race
+ * may be NULL when temperatures is NULL and temperature <= 0. workspace:
+ * zeroed once before first use and left zeroed where it has to be; one call
+ * at a time per workspace.
+ */
+size_t vasr_pa_verify_draft_tokens_workspace_size(int32_t num_seqs, int32_t num_drafts,
+                                                  int64_t vocab);
+int32_t vasr_pa_verify_draft_tokens(
+    int32_t *out_tokens, int32_t *num_accepted, const void *target_logits,
+    int64_t logits_seq_stride, int64_t logits_row_stride, int32_t dtype,
+    const int32_t *draft_tokens, const int32_t *draft_lens, const void *draft_probs,
+    int64_t probs_seq_stride, int64_t probs_row_stride, int32_t probs_dtype, const float *uniform,
+    const float *race, int64_t race_seq_stride, const float *temperatures, float temperature,
+    int32_t num_seqs, int32_t num_drafts, int64_t vocab, void *workspace, size_t workspace_bytes,
+    vasr_pa_stream_t stream);
 
 /*
  * Read (and optionally clear) the device error word of the current device.

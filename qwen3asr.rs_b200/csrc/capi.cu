@@ -534,6 +534,260 @@ int32_t vasr_pa_greedy_argmax(uint32_t *next_ids, const void *logits, int32_t nu
   return vasr::launch_greedy_argmax(a, workspace, to_stream(stream));
 }
 
+namespace {
+// Fills the rotary angles of the multi-axis entry points.
+int check_mrope(vasr::MropeAngles *r, const float *cos_table, const float *sin_table,
+                int64_t max_position, const int64_t *positions, int64_t axis_stride,
+                const int32_t *sections, int32_t num_axes, int32_t interleaved, int32_t head_dim) {
+  if (num_axes < 1 || num_axes > vasr::kMropeMaxAxes || max_position <= 0 || axis_stride < 0 || !sections)
+    return VASR_PA_EINVAL_SHAPE;
+  int64_t half = 0;
+  for (int a = 0; a < num_axes; ++a) {
+    if (sections[a] < 0) return VASR_PA_EINVAL_SHAPE;
+    half += sections[a];
+  }
+  if (half <= 0 || 2 * half > head_dim) return VASR_PA_EINVAL_SHAPE;
+  if (interleaved)  // axis a's frequencies are a, a + num_axes, ...: all of them must exist
+    for (int a = 1; a < num_axes; ++a)
+      if (sections[a] > 0 && a + (int64_t)(sections[a] - 1) * num_axes >= half) return VASR_PA_EINVAL_SHAPE;
+  if (!cos_table || !sin_table || !positions) return VASR_PA_EINVAL_POINTER;
+  if (!aligned(cos_table, 4) || !aligned(sin_table, 4) || !aligned(positions, 8)) return VASR_PA_EINVAL_ALIGN;
+  r->cos_table = cos_table;
+  r->sin_table = sin_table;
+  r->positions = positions;
+  r->axis_stride = axis_stride;
+  r->max_position = max_position;
+  r->half = (int)half;
+  r->num_axes = num_axes;
+  r->interleaved = interleaved != 0;
+  for (int a = 0; a < vasr::kMropeMaxAxes; ++a) r->sections[a] = a < num_axes ? sections[a] : 0;
+  return VASR_PA_OK;
+}
+
+// Bytes of a cache element: the query's type or fp8, 0 for any other pair.
+int cache_elem_size(int32_t dtype, int32_t cache_dtype) {
+  if (cache_dtype == VASR_PA_FP8_E4M3) return 1;
+  return cache_dtype == dtype ? elem_size(dtype) : 0;
+}
+}  // namespace
+
+int32_t vasr_pa_mrope(void *out, int64_t out_token_stride, int64_t out_head_stride, const void *x,
+                      int64_t x_token_stride, int64_t x_head_stride, const float *cos_table,
+                      const float *sin_table, int64_t max_position, const int64_t *positions,
+                      int64_t position_axis_stride, const int32_t *sections, int32_t num_axes,
+                      int32_t interleaved, int32_t inverse, int64_t num_tokens, int32_t num_heads,
+                      int32_t head_dim, int32_t dtype, vasr_pa_stream_t stream) {
+  const int es = elem_size(dtype);
+  if (es == 0) return VASR_PA_EINVAL_DTYPE;
+  if (num_tokens < 0 || num_heads <= 0 || head_dim <= 0 || x_token_stride < 0 || x_head_stride < 0 ||
+      out_token_stride < 0 || out_head_stride < 0)
+    return VASR_PA_EINVAL_SHAPE;
+  vasr::MropeArgs a{};
+  const int r = check_mrope(&a.rope, cos_table, sin_table, max_position, positions, position_axis_stride,
+                            sections, num_axes, interleaved, head_dim);
+  if (r == VASR_PA_EINVAL_SHAPE) return r;
+  if (num_tokens == 0) return VASR_PA_OK;
+  if (r != VASR_PA_OK) return r;
+  // rows of out must not overlap: [tokens, heads, dims] or [heads, tokens, dims] order
+  const bool heads_inside = out_head_stride >= head_dim && out_token_stride >= (num_heads - 1) * out_head_stride + head_dim;
+  const bool tokens_inside = out_token_stride >= head_dim && out_head_stride >= (num_tokens - 1) * out_token_stride + head_dim;
+  const bool one_head = num_heads == 1 && out_token_stride >= head_dim;
+  const bool one_token = num_tokens == 1 && (num_heads == 1 || out_head_stride >= head_dim);
+  if (!heads_inside && !tokens_inside && !one_head && !one_token) return VASR_PA_EINVAL_SHAPE;
+  if (!out || !x) return VASR_PA_EINVAL_POINTER;
+  if (!aligned(out, es) || !aligned(x, es)) return VASR_PA_EINVAL_ALIGN;
+  a.out = out;
+  a.x = x;
+  a.out_token_stride = out_token_stride;
+  a.out_head_stride = out_head_stride;
+  a.x_token_stride = x_token_stride;
+  a.x_head_stride = x_head_stride;
+  a.inverse = inverse != 0;
+  a.num_tokens = num_tokens;
+  a.num_heads = num_heads;
+  a.head_dim = head_dim;
+  a.dtype = dtype;
+  return vasr::launch_mrope(a, to_stream(stream));
+}
+
+int32_t vasr_pa_fused_qk_norm_mrope_append(
+    void *q_out, const void *qkv, int64_t qkv_token_stride, const void *q_norm_weight,
+    const void *k_norm_weight, float eps, const float *cos_table, const float *sin_table,
+    int64_t max_position, const int64_t *positions, int64_t position_axis_stride,
+    const int32_t *sections, int32_t num_axes, int32_t interleaved, void *key_cache,
+    void *value_cache, float *score_cache, const int64_t *slot_mapping, int64_t num_tokens,
+    int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+    int64_t num_blocks, int32_t dtype, int32_t cache_dtype, const float *k_scale,
+    const float *v_scale, vasr_pa_stream_t stream) {
+  const int g = check_geometry(dtype, num_kv_heads, head_dim, block_size, num_blocks);
+  if (g != VASR_PA_OK) return g;
+  const int es = elem_size(dtype), ces = cache_elem_size(dtype, cache_dtype);
+  if (ces == 0) return VASR_PA_EINVAL_DTYPE;
+  if (head_dim % (16 / ces) != 0 || num_tokens < 0 || num_heads <= 0) return VASR_PA_EINVAL_SHAPE;
+  if (head_dim > 512) return VASR_PA_ENOT_SUPPORTED;
+  vasr::MropeAppendArgs a{};
+  const int r = check_mrope(&a.rope, cos_table, sin_table, max_position, positions, position_axis_stride,
+                            sections, num_axes, interleaved, head_dim);
+  if (r == VASR_PA_EINVAL_SHAPE) return r;
+  if (num_tokens == 0) return VASR_PA_OK;
+  if (r != VASR_PA_OK) return r;
+  if (qkv_token_stride < ((int64_t)num_heads + 2 * (int64_t)num_kv_heads) * head_dim) return VASR_PA_EINVAL_SHAPE;
+  if (!q_out || !qkv || !key_cache || !value_cache || !slot_mapping || !q_norm_weight != !k_norm_weight ||
+      (cache_dtype == VASR_PA_FP8_E4M3 && (!k_scale || !v_scale)))
+    return VASR_PA_EINVAL_POINTER;
+  if (!aligned(q_out, es) || !aligned(qkv, es) || !aligned(q_norm_weight, es) || !aligned(k_norm_weight, es) ||
+      !aligned16(key_cache) || !aligned16(value_cache) || !aligned(score_cache, 4) ||
+      !aligned(slot_mapping, 8) || !aligned(k_scale, 4) || !aligned(v_scale, 4))
+    return VASR_PA_EINVAL_ALIGN;
+  a.q_out = q_out;
+  a.qkv = qkv;
+  a.qkv_token_stride = qkv_token_stride;
+  a.q_norm_weight = q_norm_weight;
+  a.k_norm_weight = k_norm_weight;
+  a.eps = eps;
+  a.key_cache = key_cache;
+  a.value_cache = value_cache;
+  a.score_cache = score_cache;
+  a.slot_mapping = slot_mapping;
+  a.num_tokens = num_tokens;
+  a.num_heads = num_heads;
+  a.num_kv_heads = num_kv_heads;
+  a.head_dim = head_dim;
+  a.block_size = block_size;
+  a.num_blocks = num_blocks;
+  a.dtype = dtype;
+  a.cache_dtype = cache_dtype;
+  a.k_scale = cache_dtype == VASR_PA_FP8_E4M3 ? k_scale : nullptr;
+  a.v_scale = cache_dtype == VASR_PA_FP8_E4M3 ? v_scale : nullptr;
+  return vasr::launch_mrope_append(a, to_stream(stream));
+}
+
+size_t vasr_pa_paged_attention_scored_workspace_size(int32_t num_seqs, int32_t query_len,
+                                                     int32_t score_rows, int32_t num_heads,
+                                                     int32_t num_kv_heads, int32_t head_dim,
+                                                     int32_t block_size, int32_t max_context_len) {
+  if (num_seqs <= 0 || query_len <= 0 || score_rows <= 0 || score_rows > query_len || num_kv_heads <= 0 ||
+      num_heads <= 0 || num_heads % num_kv_heads != 0 || head_dim <= 0 || !block_size_ok(block_size))
+    return 0;
+  return vasr::scored_workspace_bytes(num_seqs, query_len, score_rows, num_heads, num_kv_heads, head_dim,
+                                      block_size, max_context_len > 0 ? max_context_len : 1);
+}
+
+int32_t vasr_pa_paged_attention_scored(
+    void *out, const void *query, const void *key_cache, const void *value_cache,
+    float *score_cache, const uint32_t *block_tables, const uint32_t *context_lens,
+    int32_t num_seqs, int32_t query_len, int32_t score_rows, int32_t num_heads,
+    int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int64_t num_blocks,
+    int32_t max_num_blocks_per_seq, int32_t max_context_len, float scale, float softcapping,
+    float decay, int64_t q_token_stride, int32_t dtype, int32_t cache_dtype, const float *k_scale,
+    const float *v_scale, void *workspace, size_t workspace_bytes, vasr_pa_stream_t stream) {
+  const int g = check_geometry(dtype, num_kv_heads, head_dim, block_size, num_blocks);
+  if (g != VASR_PA_OK) return g;
+  const int es = elem_size(dtype), ces = cache_elem_size(dtype, cache_dtype);
+  if (ces == 0) return VASR_PA_EINVAL_DTYPE;
+  if (head_dim % (16 / ces) != 0 || num_seqs < 0 || num_heads <= 0 || num_heads % num_kv_heads != 0 ||
+      max_num_blocks_per_seq <= 0 || max_context_len < 0 || query_len <= 0 || score_rows <= 0 ||
+      score_rows > query_len)
+    return VASR_PA_EINVAL_SHAPE;
+  if (!(softcapping > 0.f) || !(decay >= 0.f && decay <= 1.f)) return VASR_PA_EINVAL_SHAPE;
+  if (head_dim > 512 || query_len > 64) return VASR_PA_ENOT_SUPPORTED;
+  if (num_seqs == 0) return VASR_PA_OK;
+  if (num_seqs > 65535 || num_heads > 65535 || q_token_stride < (int64_t)num_heads * head_dim)
+    return VASR_PA_EINVAL_SHAPE;
+  if (!out || !query || !key_cache || !value_cache || !score_cache || !block_tables || !context_lens ||
+      (cache_dtype == VASR_PA_FP8_E4M3 && (!k_scale || !v_scale)))
+    return VASR_PA_EINVAL_POINTER;
+  if (!aligned16(query) || !aligned16(key_cache) || !aligned16(value_cache) || !aligned(score_cache, 4) ||
+      (q_token_stride * es) % 16 != 0 || !aligned(out, es) || !aligned(block_tables, 4) ||
+      !aligned(context_lens, 4) || (workspace && !aligned(workspace, 256)) || !aligned(k_scale, 4) ||
+      !aligned(v_scale, 4))
+    return VASR_PA_EINVAL_ALIGN;
+  const int ctx = max_context_len > 0 ? max_context_len : 1;
+  if (!workspace || workspace_bytes < vasr::scored_workspace_bytes(num_seqs, query_len, score_rows, num_heads,
+                                                                   num_kv_heads, head_dim, block_size, ctx))
+    return VASR_PA_EINVAL_WORKSPACE;
+  const bool fp8 = cache_dtype == VASR_PA_FP8_E4M3;
+  vasr::ScoredArgs a{out, query, key_cache, value_cache, score_cache, block_tables, context_lens, num_seqs,
+                     query_len, score_rows, num_heads, num_kv_heads, head_dim, block_size, num_blocks,
+                     max_num_blocks_per_seq, ctx, scale, softcapping, decay, q_token_stride, dtype,
+                     cache_dtype, fp8 ? k_scale : nullptr, fp8 ? v_scale : nullptr, workspace,
+                     workspace_bytes};
+  return vasr::launch_scored(a, to_stream(stream));
+}
+
+int32_t vasr_pa_evict_kv(void *key_cache, void *value_cache, float *score_cache,
+                         const uint32_t *block_tables, int32_t max_num_blocks_per_seq,
+                         const uint32_t *out_block_tables, int32_t out_max_num_blocks_per_seq,
+                         const uint32_t *context_lens, int32_t max_context_len,
+                         const uint32_t *budgets, int32_t budget, int32_t num_sink,
+                         int32_t num_recent, int32_t *kept, uint32_t *new_lens, int32_t num_seqs,
+                         int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                         int64_t num_blocks, int32_t dtype, vasr_pa_stream_t stream) {
+  const int es = dtype == VASR_PA_FP8_E4M3 ? 1 : elem_size(dtype);
+  if (es == 0) return VASR_PA_EINVAL_DTYPE;
+  if (!block_size_ok(block_size)) return VASR_PA_EINVAL_BLOCKSIZE;
+  if (num_kv_heads <= 0 || head_dim <= 0 || num_blocks <= 0 || head_dim % (16 / es) != 0 || num_seqs < 0 ||
+      max_num_blocks_per_seq <= 0 || max_context_len <= 0 || budget <= 0 || num_sink < 0 || num_recent < 0 ||
+      (int64_t)num_sink + num_recent > budget || (out_block_tables && out_max_num_blocks_per_seq <= 0))
+    return VASR_PA_EINVAL_SHAPE;
+  if (out_block_tables) {  // the longest result has to fit
+    const int64_t longest = budget < max_context_len ? budget : max_context_len;
+    if ((int64_t)out_max_num_blocks_per_seq * block_size < longest) return VASR_PA_EINVAL_SHAPE;
+  }
+  if (num_seqs == 0) return VASR_PA_OK;
+  if (num_seqs > 65535 || num_kv_heads > 65535) return VASR_PA_EINVAL_SHAPE;
+  if (!key_cache || !value_cache || !score_cache || !block_tables || !context_lens || !kept || !new_lens)
+    return VASR_PA_EINVAL_POINTER;
+  if (!aligned16(key_cache) || !aligned16(value_cache) || !aligned(score_cache, 4) || !aligned(block_tables, 4) ||
+      !aligned(out_block_tables, 4) || !aligned(context_lens, 4) || !aligned(budgets, 4) || !aligned(kept, 4) ||
+      !aligned(new_lens, 4))
+    return VASR_PA_EINVAL_ALIGN;
+  vasr::EvictArgs a{key_cache, value_cache, score_cache, block_tables, out_block_tables, context_lens, budgets,
+                    kept, new_lens, max_context_len, budget, num_sink, num_recent, num_seqs, num_kv_heads,
+                    head_dim, block_size, num_blocks, max_num_blocks_per_seq, out_max_num_blocks_per_seq, es};
+  return vasr::launch_evict(a, to_stream(stream));
+}
+
+size_t vasr_pa_verify_draft_tokens_workspace_size(int32_t num_seqs, int32_t num_drafts,
+                                                  int64_t vocab) {
+  if (num_seqs <= 0 || num_drafts < 0 || vocab <= 0) return 0;
+  return vasr::verify_workspace_bytes(num_seqs, num_drafts, vocab);
+}
+
+int32_t vasr_pa_verify_draft_tokens(
+    int32_t *out_tokens, int32_t *num_accepted, const void *target_logits,
+    int64_t logits_seq_stride, int64_t logits_row_stride, int32_t dtype,
+    const int32_t *draft_tokens, const int32_t *draft_lens, const void *draft_probs,
+    int64_t probs_seq_stride, int64_t probs_row_stride, int32_t probs_dtype, const float *uniform,
+    const float *race, int64_t race_seq_stride, const float *temperatures, float temperature,
+    int32_t num_seqs, int32_t num_drafts, int64_t vocab, void *workspace, size_t workspace_bytes,
+    vasr_pa_stream_t stream) {
+  const int es = elem_size(dtype);
+  if (es == 0 || (draft_probs && elem_size(probs_dtype) == 0)) return VASR_PA_EINVAL_DTYPE;
+  if (num_seqs < 0 || num_seqs > 65535 || num_drafts < 0 || num_drafts > 1023 || vocab <= 0 ||
+      vocab > 0x7fffffffLL || logits_seq_stride < 0 || race_seq_stride < 0 || probs_seq_stride < 0 ||
+      (num_drafts > 0 && logits_row_stride < vocab) ||
+      (draft_probs && num_drafts > 1 && probs_row_stride < vocab))
+    return VASR_PA_EINVAL_SHAPE;
+  if (num_seqs == 0) return VASR_PA_OK;
+  const bool greedy = !temperatures && !(temperature > 0.f);
+  if (!out_tokens || !num_accepted || !target_logits || (num_drafts > 0 && !draft_tokens) ||
+      (!greedy && (!race || (num_drafts > 0 && !uniform))))
+    return VASR_PA_EINVAL_POINTER;
+  if (!aligned(target_logits, es) || !aligned(out_tokens, 4) || !aligned(num_accepted, 4) ||
+      !aligned(draft_tokens, 4) || !aligned(draft_lens, 4) ||
+      (draft_probs && !aligned(draft_probs, elem_size(probs_dtype))) || !aligned(uniform, 4) ||
+      !aligned(race, 4) || !aligned(temperatures, 4) || (workspace && !aligned(workspace, 256)))
+    return VASR_PA_EINVAL_ALIGN;
+  if (!workspace || workspace_bytes < vasr::verify_workspace_bytes(num_seqs, num_drafts, vocab))
+    return VASR_PA_EINVAL_WORKSPACE;
+  vasr::VerifyArgs a{out_tokens, num_accepted, target_logits, logits_seq_stride, logits_row_stride, dtype,
+                     draft_tokens, draft_lens, draft_probs, probs_seq_stride, probs_row_stride, probs_dtype,
+                     uniform, race, race_seq_stride, temperatures, temperature, num_seqs, num_drafts, vocab,
+                     workspace};
+  return vasr::launch_verify(a, to_stream(stream));
+}
+
 int32_t vasr_pa_get_device_error(int32_t *out_bits, int32_t clear, vasr_pa_stream_t stream) {
   if (!out_bits) return VASR_PA_EINVAL_POINTER;
   uint32_t a = 0, b = 0, c = 0, d = 0, e = 0;
@@ -546,7 +800,11 @@ int32_t vasr_pa_get_device_error(int32_t *out_bits, int32_t clear, vasr_pa_strea
     return r;
   uint32_t f = 0;
   if ((r = vasr::read_error_decode_loop(&f, clear != 0, to_stream(stream))) != VASR_PA_OK) return r;
-  *out_bits = (int32_t)(a | b | c | d | e | f);
+  uint32_t g = 0, h = 0, i = 0;
+  if ((r = vasr::read_error_mrope(&g, clear != 0, to_stream(stream))) != VASR_PA_OK) return r;
+  if ((r = vasr::read_error_scored(&h, clear != 0, to_stream(stream))) != VASR_PA_OK) return r;
+  if ((r = vasr::read_error_evict(&i, clear != 0, to_stream(stream))) != VASR_PA_OK) return r;
+  *out_bits = (int32_t)(a | b | c | d | e | f | g | h | i);
   return VASR_PA_OK;
 }
 

@@ -129,6 +129,150 @@ struct FusedRopeArgs {
 };
 int launch_fused_rope(const FusedRopeArgs &a, cudaStream_t s);
 
+// Rotary angles of several position axes (mrope.cu). sections[a] of the half
+// frequencies belong to axis a, one section after another or interleaved.
+constexpr int kMropeMaxAxes = 4;
+struct MropeAngles {
+  const float *cos_table;  // [max_position, half]
+  const float *sin_table;
+  const int64_t *positions;  // axis a of token t at positions[a * axis_stride + t]
+  int64_t axis_stride;
+  int64_t max_position;
+  int half;
+  int num_axes;
+  int interleaved;
+  int sections[kMropeMaxAxes];
+};
+
+struct MropeAppendArgs {
+  void *q_out;
+  const void *qkv;
+  int64_t qkv_token_stride;
+  const void *q_norm_weight;  // both null: no norm
+  const void *k_norm_weight;
+  float eps;
+  MropeAngles rope;
+  void *key_cache;
+  void *value_cache;
+  float *score_cache;  // may be null; else cleared at every appended slot
+  const int64_t *slot_mapping;
+  int64_t num_tokens;
+  int num_heads;
+  int num_kv_heads;
+  int head_dim;
+  int block_size;
+  int64_t num_blocks;
+  int dtype;
+  int cache_dtype;       // dtype or VASR_PA_FP8_E4M3
+  const float *k_scale;  // fp8 pages: device scalars
+  const float *v_scale;
+};
+int launch_mrope_append(const MropeAppendArgs &a, cudaStream_t s);
+
+struct MropeArgs {
+  void *out;
+  const void *x;
+  int64_t out_token_stride, out_head_stride;
+  int64_t x_token_stride, x_head_stride;
+  MropeAngles rope;
+  int inverse;
+  int64_t num_tokens;
+  int num_heads;
+  int head_dim;
+  int dtype;
+};
+int launch_mrope(const MropeArgs &a, cudaStream_t s);
+int read_error_mrope(uint32_t *bits, bool clear, cudaStream_t s);
+
+// Decode attention over a window of query_len rows a sequence that adds every
+// visible token's weight to its score (scored.cu).
+struct ScoredArgs {
+  void *out;
+  const void *query;
+  const void *key_cache;
+  const void *value_cache;
+  float *score_cache;  // [num_blocks, num_kv_heads, block_size]
+  const uint32_t *block_tables;
+  const uint32_t *context_lens;
+  int num_seqs;
+  int query_len;
+  int score_rows;
+  int num_heads;
+  int num_kv_heads;
+  int head_dim;
+  int block_size;
+  int64_t num_blocks;
+  int max_num_blocks_per_seq;
+  int max_context_len;
+  float scale;
+  float softcapping;
+  float decay;
+  int64_t q_token_stride;
+  int dtype;
+  int cache_dtype;
+  const float *k_scale;
+  const float *v_scale;
+  void *workspace;
+  size_t workspace_bytes;
+};
+size_t scored_workspace_bytes(int num_seqs, int query_len, int score_rows, int num_heads,
+                              int num_kv_heads, int head_dim, int block_size, int max_context_len);
+int launch_scored(const ScoredArgs &a, cudaStream_t s);
+int read_error_scored(uint32_t *bits, bool clear, cudaStream_t s);
+
+// Selection of the tokens that stay in the cache and their move to the front
+// of the sequence's pages (evict.cu).
+struct EvictArgs {
+  void *key_cache;
+  void *value_cache;
+  float *score_cache;
+  const uint32_t *block_tables;
+  const uint32_t *out_block_tables;  // null: in place
+  const uint32_t *context_lens;
+  const uint32_t *budgets;  // may be null: budget for every sequence
+  int32_t *kept;            // [num_seqs, num_kv_heads, budget]
+  uint32_t *new_lens;
+  int max_context_len;
+  int budget;
+  int num_sink;
+  int num_recent;
+  int num_seqs;
+  int num_kv_heads;
+  int head_dim;
+  int block_size;
+  int64_t num_blocks;
+  int cols;
+  int out_cols;
+  int elem_size;
+};
+int launch_evict(const EvictArgs &a, cudaStream_t s);
+int read_error_evict(uint32_t *bits, bool clear, cudaStream_t s);
+
+// Acceptance of drafted tokens and the token that follows (verify.cu).
+struct VerifyArgs {
+  int32_t *out_tokens;    // [num_seqs, num_drafts + 1]
+  int32_t *num_accepted;  // [num_seqs]
+  const void *logits;
+  int64_t logits_seq_stride, logits_row_stride;
+  int dtype;
+  const int32_t *draft_tokens;
+  const int32_t *draft_lens;  // may be null: num_drafts each
+  const void *draft_probs;    // may be null: the drafter was certain
+  int64_t probs_seq_stride, probs_row_stride;
+  int probs_dtype;
+  const float *uniform;  // [num_seqs, num_drafts]
+  const float *race;     // [num_seqs, vocab]
+  int64_t race_seq_stride;
+  const float *temperatures;  // may be null: temperature for every sequence
+  float temperature;
+  int num_seqs;
+  int num_drafts;
+  int64_t vocab;
+  void *workspace;
+};
+size_t verify_workspace_bytes(int num_seqs, int num_drafts, int64_t vocab);
+int launch_verify(const VerifyArgs &a, cudaStream_t s);
+
 struct DecodeStepArgs {
   const uint32_t *next_ids;
   const uint32_t *eos_ids;

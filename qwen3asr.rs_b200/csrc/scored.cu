@@ -1,0 +1,238 @@
+// scored.cu — paged attention of a few new tokens that also accumulates every
+// cached token's attention weight.
+//
+// Row (i, head) of sequence b, i < query_len, sits at position
+// len_b - query_len + i and sees the tokens up to there (a row before the
+// first token sees none and gives zeros):
+//   x_j = scale q . k_j   (softcapped when asked),  p_j = softmax(x)_j,
+//   out = sum_j p_j v_j,
+//   score_j <- decay score_j + sum over i < score_rows and the kv head's query
+//              heads of p_j                       for every j < len_b.
+// The weights need the whole row's maximum and sum, which a split of the
+// context does not have: each split leaves its raw scores x (log2 domain) and
+// its partial (o, m, l) in the workspace, a merge makes out and the final
+// (m, l) of every row, and the last step turns the raw scores into weights.
+#include "common.cuh"
+#include "launch.h"
+
+namespace vasr {
+namespace {
+
+constexpr int kSplitTokens = 256;
+constexpr int kThreads = 128;
+constexpr int kMergeThreads = 128;
+constexpr int kWeightThreads = 256;
+
+struct ScoredLayout {
+  int splits;         // of max_context_len
+  int64_t x_stride;   // raw scores of one row
+  size_t off_o, off_ml, off_x, total;
+};
+
+size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+
+ScoredLayout layout(int num_seqs, int query_len, int score_rows, int num_heads, int num_kv_heads,
+                    int head_dim, int max_context_len) {
+  ScoredLayout l;
+  l.splits = (max_context_len + kSplitTokens - 1) / kSplitTokens;
+  l.x_stride = (int64_t)l.splits * kSplitTokens;
+  const size_t rows = (size_t)num_seqs * query_len * num_heads;
+  l.off_o = 0;
+  l.off_ml = align256(rows * l.splits * head_dim * sizeof(float));
+  l.off_x = align256(l.off_ml + rows * (l.splits + 1) * sizeof(float2));
+  l.total = l.off_x + align256((size_t)num_seqs * score_rows * num_heads * l.x_stride * sizeof(float));
+  (void)num_kv_heads;
+  return l;
+}
+
+struct ScoredParams {
+  ScoredArgs a;
+  float *o;       // [row][split][D]
+  float2 *ml;     // [row][split], the merged one at [row][splits]
+  float *x;       // [scored row][x_stride]
+  int splits;
+  int64_t x_stride;
+  int group;      // query heads per kv head
+};
+
+__device__ __forceinline__ int context_of(const ScoredArgs &a, int b) {
+  int64_t n = a.context_lens[b];
+  const int64_t cap = min((int64_t)a.max_num_blocks_per_seq * a.block_size, (int64_t)a.max_context_len);
+  if (n > cap) {
+    raise_device_error(VASR_PA_DERR_CTX_RANGE);
+    n = cap;
+  }
+  return (int)n;
+}
+__device__ __forceinline__ int64_t page_of(const ScoredArgs &a, int b, int j) {
+  const uint32_t id = a.block_tables[(int64_t)b * a.max_num_blocks_per_seq + j / a.block_size];
+  if ((int64_t)id < a.num_blocks) return id;
+  raise_device_error(VASR_PA_DERR_BLOCK_RANGE);
+  return 0;
+}
+// Row r = (i, head): i * num_heads + head.
+__device__ __forceinline__ int64_t row_index(const ScoredArgs &a, int b, int i, int head) {
+  return ((int64_t)b * a.query_len + i) * a.num_heads + head;
+}
+
+__device__ __forceinline__ float block_reduce(float v, bool is_max) {
+  __shared__ float part[kThreads / 32];
+  v = is_max ? warp_max_xor(v, 32) : warp_sum_xor(v, 32);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = part[0];
+  for (int w = 1; w < kThreads / 32; ++w) v = is_max ? fmaxf(v, part[w]) : v + part[w];
+  __syncthreads();
+  return v;
+}
+
+// One (split, query head, sequence): every row of the window over the split.
+template <typename T, typename TC>
+__global__ void __launch_bounds__(kThreads) scored_split_kernel(const ScoredParams p) {
+  const ScoredArgs &a = p.a;
+  const int split = blockIdx.x, head = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+  const int D = a.head_dim, BS = a.block_size, kvh = head / p.group;
+  constexpr int kX = Elem<TC>::kX;
+  extern __shared__ float smem[];
+  float *q = smem, *w = smem + D;
+  const int n = context_of(a, b);
+  const int t0 = split * kSplitTokens;
+  if (t0 >= n) return;
+  const int t1 = min(n, t0 + kSplitTokens);
+  const TC *kc = static_cast<const TC *>(a.key_cache);
+  const TC *vc = static_cast<const TC *>(a.value_cache);
+  const float k_mul = a.k_scale ? a.scale * __ldg(a.k_scale) : a.scale;
+  for (int i = 0; i < a.query_len; ++i) {
+    const int64_t row = row_index(a, b, i, head);
+    const int seen = min(t1, n - a.query_len + i + 1);  // tokens [t0, seen) are visible
+    const T *qp = static_cast<const T *>(a.query) + ((int64_t)b * a.query_len + i) * a.q_token_stride + (int64_t)head * D;
+    for (int d = tid; d < D; d += kThreads) q[d] = Elem<T>::to_f32(qp[d]);
+    __syncthreads();
+    float *x = nullptr;
+    if (i < a.score_rows) x = p.x + (((int64_t)b * a.score_rows + i) * a.num_heads + head) * p.x_stride;
+    float m = -INFINITY;
+    for (int j = t0 + tid; j < t1; j += kThreads) {
+      float s = -INFINITY;
+      if (j < seen) {
+        const TC *k = kc + (page_of(a, b, j) * a.num_kv_heads + kvh) * (int64_t)D * BS + (j % BS) * kX;
+        float dot = 0.f;
+        for (int c = 0; c < D / kX; ++c) {
+          float f[kX];
+          unpack_chunk<TC>(*reinterpret_cast<const uint4 *>(k + (int64_t)c * BS * kX), f);
+#pragma unroll
+          for (int e = 0; e < kX; ++e) dot = fmaf(q[c * kX + e], f[e], dot);
+        }
+        s = dot * k_mul;
+        if (a.softcapping != 1.f) s = a.softcapping * tanhf(s / a.softcapping);
+        s *= kLog2e;
+      }
+      if (x) x[j] = s;
+      w[j - t0] = s;
+      m = fmaxf(m, s);
+    }
+    m = block_reduce(m, true);
+    float l = 0.f;
+    for (int j = t0 + tid; j < t1; j += kThreads) {
+      const float e = w[j - t0] == -INFINITY ? 0.f : exp2f(w[j - t0] - m);
+      w[j - t0] = e;
+      l += e;
+    }
+    l = block_reduce(l, false);
+    for (int d = tid; d < D; d += kThreads) {
+      float o = 0.f;
+      for (int j = t0; j < seen; ++j) {
+        const TC *v = vc + (page_of(a, b, j) * a.num_kv_heads + kvh) * (int64_t)D * BS;
+        o = fmaf(w[j - t0], Elem<TC>::to_f32(v[(int64_t)d * BS + j % BS]), o);
+      }
+      p.o[(row * p.splits + split) * D + d] = o;
+    }
+    if (tid == 0) p.ml[row * (p.splits + 1) + split] = make_float2(m, l);
+    __syncthreads();
+  }
+}
+
+// One row: the splits' partials into out and the row's final (m, l).
+template <typename T>
+__global__ void __launch_bounds__(kMergeThreads) scored_merge_kernel(const ScoredParams p) {
+  const ScoredArgs &a = p.a;
+  const int64_t row = blockIdx.x;
+  const int b = (int)(row / ((int64_t)a.query_len * a.num_heads));
+  const int n = context_of(a, b);
+  const int splits = (n + kSplitTokens - 1) / kSplitTokens;
+  const float2 *ml = p.ml + row * (p.splits + 1);
+  float m = -INFINITY, l = 0.f;
+  for (int s = 0; s < splits; ++s) m = fmaxf(m, ml[s].x);
+  for (int s = 0; s < splits; ++s)
+    if (ml[s].y != 0.f) l = fmaf(ml[s].y, exp2f(ml[s].x - m), l);
+  const float v_mul = a.v_scale ? __ldg(a.v_scale) : 1.f;
+  for (int d = threadIdx.x; d < a.head_dim; d += kMergeThreads) {
+    float o = 0.f;
+    for (int s = 0; s < splits; ++s)
+      if (ml[s].y != 0.f) o = fmaf(p.o[(row * p.splits + s) * a.head_dim + d], exp2f(ml[s].x - m), o);
+    static_cast<T *>(a.out)[row * a.head_dim + d] = Elem<T>::from_f32(l != 0.f ? o / l * v_mul : 0.f);
+  }
+  if (threadIdx.x == 0) p.ml[row * (p.splits + 1) + p.splits] = make_float2(m, l);
+}
+
+// The weights of the scored rows, added to the tokens' scores.
+__global__ void __launch_bounds__(kWeightThreads) scored_weight_kernel(const ScoredParams p) {
+  const ScoredArgs &a = p.a;
+  const int kvh = blockIdx.y, b = blockIdx.z;
+  const int n = context_of(a, b);
+  const int j = blockIdx.x * kWeightThreads + threadIdx.x;
+  if (j >= n) return;
+  float sum = 0.f;
+  for (int i = 0; i < a.score_rows; ++i)
+    for (int g = 0; g < p.group; ++g) {
+      const int head = kvh * p.group + g;
+      const float2 ml = p.ml[row_index(a, b, i, head) * (p.splits + 1) + p.splits];
+      const float x = p.x[(((int64_t)b * a.score_rows + i) * a.num_heads + head) * p.x_stride + j];
+      if (ml.y != 0.f) sum += exp2f(x - ml.x) / ml.y;
+    }
+  float *s = a.score_cache + (page_of(a, b, j) * a.num_kv_heads + kvh) * a.block_size + j % a.block_size;
+  *s = a.decay * *s + sum;
+}
+
+template <typename T, typename TC>
+int launch_scored_t(const ScoredArgs &a, cudaStream_t s) {
+  const ScoredLayout l = layout(a.num_seqs, a.query_len, a.score_rows, a.num_heads, a.num_kv_heads,
+                                a.head_dim, a.max_context_len);
+  unsigned char *ws = static_cast<unsigned char *>(a.workspace);
+  ScoredParams p{a, reinterpret_cast<float *>(ws + l.off_o), reinterpret_cast<float2 *>(ws + l.off_ml),
+                 reinterpret_cast<float *>(ws + l.off_x), l.splits, l.x_stride, a.num_heads / a.num_kv_heads};
+  const int64_t rows = (int64_t)a.num_seqs * a.query_len * a.num_heads;
+  if (rows > 0x7fffffff) return VASR_PA_EINVAL_SHAPE;
+  scored_split_kernel<T, TC><<<dim3((unsigned)l.splits, (unsigned)a.num_heads, (unsigned)a.num_seqs), kThreads,
+                               (a.head_dim + kSplitTokens) * sizeof(float), s>>>(p);
+  scored_merge_kernel<T><<<(unsigned)rows, kMergeThreads, 0, s>>>(p);
+  const unsigned chunks = (unsigned)((a.max_context_len + kWeightThreads - 1) / kWeightThreads);
+  scored_weight_kernel<<<dim3(chunks, (unsigned)a.num_kv_heads, (unsigned)a.num_seqs), kWeightThreads, 0, s>>>(p);
+  return cudaPeekAtLastError() == cudaSuccess ? VASR_PA_OK : VASR_PA_ELAUNCH;
+}
+
+template <typename T>
+int launch_scored_c(const ScoredArgs &a, cudaStream_t s) {
+  if (a.cache_dtype == VASR_PA_FP8_E4M3) return launch_scored_t<T, __nv_fp8_e4m3>(a, s);
+  return launch_scored_t<T, T>(a, s);
+}
+
+}  // namespace
+
+size_t scored_workspace_bytes(int num_seqs, int query_len, int score_rows, int num_heads, int num_kv_heads,
+                              int head_dim, int block_size, int max_context_len) {
+  (void)block_size;
+  return layout(num_seqs, query_len, score_rows, num_heads, num_kv_heads, head_dim, max_context_len).total;
+}
+
+int launch_scored(const ScoredArgs &a, cudaStream_t s) {
+  switch (a.dtype) {
+    case VASR_PA_F32: return launch_scored_c<float>(a, s);
+    case VASR_PA_BF16: return launch_scored_c<__nv_bfloat16>(a, s);
+    case VASR_PA_F16: return launch_scored_c<__half>(a, s);
+    default: return VASR_PA_EINVAL_DTYPE;
+  }
+}
+
+int read_error_scored(uint32_t *bits, bool clear, cudaStream_t s) { return read_unit_error(bits, clear, s); }
+
+}  // namespace vasr

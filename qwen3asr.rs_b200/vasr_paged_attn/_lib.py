@@ -34,6 +34,7 @@ DERR_CTX_RANGE = 0x4
 DERR_WAIT_TIMEOUT = 0x8
 DERR_MAPPING_RANGE = 0x10
 DERR_QLEN_RANGE = 0x20
+DERR_POSITION_RANGE = 0x40
 
 _c_void_p = ctypes.c_void_p
 _i32 = ctypes.c_int32
@@ -126,6 +127,39 @@ SIGNATURES: dict[str, tuple] = {
         _i32,
         [_c_void_p, _c_void_p, _i32, _i64, _i64, _i32, _c_void_p, _c_void_p, _c_void_p, _size,
          _c_void_p],
+    ),
+    "vasr_pa_mrope": (
+        _i32,
+        [_c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i64, _c_void_p, _i64,
+         _c_void_p, _i32, _i32, _i32, _i64, _i32, _i32, _i32, _c_void_p],
+    ),
+    "vasr_pa_fused_qk_norm_mrope_append": (
+        _i32,
+        [_c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p, _f32, _c_void_p, _c_void_p, _i64,
+         _c_void_p, _i64, _c_void_p, _i32, _i32, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64,
+         _i32, _i32, _i32, _i32, _i64, _i32, _i32, _c_void_p, _c_void_p, _c_void_p],
+    ),
+    "vasr_pa_paged_attention_scored_workspace_size": (
+        _size, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32]
+    ),
+    "vasr_pa_paged_attention_scored": (
+        _i32,
+        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _i32,
+         _i32, _i32, _i32, _i32, _i32, _i64, _i32, _i32, _f32, _f32, _f32, _i64, _i32, _i32,
+         _c_void_p, _c_void_p, _c_void_p, _size, _c_void_p],
+    ),
+    "vasr_pa_evict_kv": (
+        _i32,
+        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _c_void_p, _i32, _c_void_p, _i32,
+         _c_void_p, _i32, _i32, _i32, _c_void_p, _c_void_p, _i32, _i32, _i32, _i32, _i64, _i32,
+         _c_void_p],
+    ),
+    "vasr_pa_verify_draft_tokens_workspace_size": (_size, [_i32, _i32, _i64]),
+    "vasr_pa_verify_draft_tokens": (
+        _i32,
+        [_c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i32, _c_void_p, _c_void_p, _c_void_p, _i64,
+         _i64, _i32, _c_void_p, _c_void_p, _i64, _c_void_p, _f32, _i32, _i32, _i64, _c_void_p,
+         _size, _c_void_p],
     ),
 }
 

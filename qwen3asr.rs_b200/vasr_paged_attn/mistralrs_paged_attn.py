@@ -143,6 +143,29 @@ def reserve_paged_attention_workspace(device: torch.device, nbytes: int,
     return ws
 
 
+class StreamWorkspaces:
+    """One growing, zero-filled workspace per (device, stream) for one kind of call."""
+
+    def __init__(self, what: str):
+        self._what = what
+        self._held: dict[tuple[int, int], torch.Tensor] = {}
+
+    def reserve(self, device: torch.device, nbytes: int,
+                stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+        """The workspace of ``stream`` (default: the current one), at least ``nbytes`` long; call it
+        before a CUDA-graph capture that needs more than earlier calls did."""
+        s = stream if stream is not None else torch.cuda.current_stream(device)
+        key = (device.index if device.index is not None else torch.cuda.current_device(), s.cuda_stream)
+        ws = self._held.get(key)
+        if ws is None or ws.numel() < nbytes:
+            if torch.cuda.is_current_stream_capturing():
+                raise _lib.VasrPaError(_lib.EINVAL_WORKSPACE,
+                                       f"{self._what} workspace must be reserved before CUDA graph capture")
+            ws = torch.zeros(max(nbytes, 1 << 16), dtype=torch.uint8, device=device)
+            self._held[key] = ws
+        return ws
+
+
 _PREFILL_SCRATCH: dict[tuple[int, int], torch.Tensor] = {}
 
 
