@@ -697,7 +697,7 @@ int32_t vasr_pa_paged_attention_scored(
   if (!out || !query || !key_cache || !value_cache || !score_cache || !block_tables || !context_lens ||
       (cache_dtype == VASR_PA_FP8_E4M3 && (!k_scale || !v_scale)))
     return VASR_PA_EINVAL_POINTER;
-  if (!aligned16(query) || !aligned16(key_cache) || !aligned16(value_cache) || !aligned(score_cache, 4) ||
+  if (!aligned16(query) || !aligned16(key_cache) || !aligned16(value_cache) || !aligned16(score_cache) ||
       (q_token_stride * es) % 16 != 0 || !aligned(out, es) || !aligned(block_tables, 4) ||
       !aligned(context_lens, 4) || (workspace && !aligned(workspace, 256)) || !aligned(k_scale, 4) ||
       !aligned(v_scale, 4))

@@ -12,8 +12,11 @@
 // context does not have: each split leaves its raw scores x (log2 domain) and
 // its partial (o, m, l) in the workspace, a merge makes out and the final
 // (m, l) of every row, and the last step turns the raw scores into weights.
+// 16-bit queries at head_dim 128 run scored_mma_kernel (scored_mma.cuh); the
+// kernels here serve f32 and the other shapes.
 #include "common.cuh"
 #include "launch.h"
+#include "scored_mma.cuh"
 
 namespace vasr {
 namespace {
@@ -23,25 +26,64 @@ constexpr int kThreads = 128;
 constexpr int kMergeThreads = 128;
 constexpr int kWeightThreads = 256;
 
+size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+
+// Arrival counters of the tensor-core kernel: a fixed region that every call
+// leaves at zero, so that one zeroed workspace serves calls of any shape.
+constexpr int64_t kMaxCounters = 65536;
+constexpr size_t kCounterBytes = kMaxCounters * sizeof(uint32_t);
+
+// ---- tensor-core kernel: which calls it takes, its splits and its workspace
+bool takes_mma(const ScoredArgs &a) {
+  return a.dtype != VASR_PA_F32 && a.head_dim == kScoredDim &&
+         a.query_len * (a.num_heads / a.num_kv_heads) <= kScoredMaxRows &&
+         !(a.cache_dtype == VASR_PA_FP8_E4M3 && a.block_size < 16) &&
+         (int64_t)a.num_kv_heads * ((a.query_len * (a.num_heads / a.num_kv_heads) + 7) / 8) <= 65535;
+}
+
+constexpr int kMmaSplitTokens = 1024;
+constexpr int kMmaFusedContext = 4096;
+
+struct MmaLayout {
+  int pages_per_split, max_splits;
+  int64_t x_stride;
+  size_t off_counters, off_o, off_ml, off_x, total;
+};
+MmaLayout mma_layout(int num_seqs, int query_len, int score_rows, int num_heads, int num_kv_heads, int block_size,
+                     int max_context_len) {
+  MmaLayout l;
+  // halve the splits until the grid has two CTAs per SM
+  int tokens = kMmaSplitTokens;
+  while (tokens > 64 && (int64_t)num_seqs * num_kv_heads * ((max_context_len + tokens - 1) / tokens) < 2 * 148) tokens >>= 1;
+  l.pages_per_split = tokens / block_size < 1 ? 1 : tokens / block_size;
+  if (l.pages_per_split > kScoredMaxPages) l.pages_per_split = kScoredMaxPages;
+  const int per = l.pages_per_split * block_size;
+  l.max_splits = (max_context_len + per - 1) / per;
+  l.x_stride = (int64_t)l.max_splits * per;
+  const size_t rows = (size_t)num_seqs * num_kv_heads * l.max_splits * query_len * (num_heads / num_kv_heads);
+  l.off_counters = 0;
+  l.off_o = kCounterBytes;
+  l.off_ml = align256(l.off_o + rows * kScoredDim * sizeof(float));
+  l.off_x = align256(l.off_ml + rows * sizeof(float2));
+  l.total = l.off_x + align256((size_t)num_seqs * score_rows * num_heads * l.x_stride * sizeof(float));
+  return l;
+}
+
+// ---- the other kernels
 struct ScoredLayout {
   int splits;         // of max_context_len
   int64_t x_stride;   // raw scores of one row
   size_t off_o, off_ml, off_x, total;
 };
-
-size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
-
-ScoredLayout layout(int num_seqs, int query_len, int score_rows, int num_heads, int num_kv_heads,
-                    int head_dim, int max_context_len) {
+ScoredLayout layout(int num_seqs, int query_len, int score_rows, int num_heads, int head_dim, int max_context_len) {
   ScoredLayout l;
   l.splits = (max_context_len + kSplitTokens - 1) / kSplitTokens;
   l.x_stride = (int64_t)l.splits * kSplitTokens;
   const size_t rows = (size_t)num_seqs * query_len * num_heads;
-  l.off_o = 0;
-  l.off_ml = align256(rows * l.splits * head_dim * sizeof(float));
+  l.off_o = kCounterBytes;
+  l.off_ml = align256(l.off_o + rows * l.splits * head_dim * sizeof(float));
   l.off_x = align256(l.off_ml + rows * (l.splits + 1) * sizeof(float2));
   l.total = l.off_x + align256((size_t)num_seqs * score_rows * num_heads * l.x_stride * sizeof(float));
-  (void)num_kv_heads;
   return l;
 }
 
@@ -195,8 +237,8 @@ __global__ void __launch_bounds__(kWeightThreads) scored_weight_kernel(const Sco
 
 template <typename T, typename TC>
 int launch_scored_t(const ScoredArgs &a, cudaStream_t s) {
-  const ScoredLayout l = layout(a.num_seqs, a.query_len, a.score_rows, a.num_heads, a.num_kv_heads,
-                                a.head_dim, a.max_context_len);
+  const ScoredLayout l =
+      layout(a.num_seqs, a.query_len, a.score_rows, a.num_heads, a.head_dim, a.max_context_len);
   unsigned char *ws = static_cast<unsigned char *>(a.workspace);
   ScoredParams p{a, reinterpret_cast<float *>(ws + l.off_o), reinterpret_cast<float2 *>(ws + l.off_ml),
                  reinterpret_cast<float *>(ws + l.off_x), l.splits, l.x_stride, a.num_heads / a.num_kv_heads};
@@ -210,8 +252,82 @@ int launch_scored_t(const ScoredArgs &a, cudaStream_t s) {
   return cudaPeekAtLastError() == cudaSuccess ? VASR_PA_OK : VASR_PA_ELAUNCH;
 }
 
+template <typename T, typename TC, int BS, int NRT, bool kDup>
+int launch_mma_rows(const ScoredArgs &a, cudaStream_t s) {
+  constexpr int kStage = 2 * (BS < 16 ? 16 : BS) * kScoredDim * (int)sizeof(TC);
+  constexpr int kNST = kStage <= 4096 ? 8 : kStage <= 8192 ? 8 : 4;
+  constexpr int kMinB = sizeof(TC) == 1 && NRT == 1 ? 4 : 3;
+  using C = ScoredCfg<TC, BS, kNST>;
+  const MmaLayout l = mma_layout(a.num_seqs, a.query_len, a.score_rows, a.num_heads, a.num_kv_heads, a.block_size,
+                                 a.max_context_len);
+  unsigned char *ws = static_cast<unsigned char *>(a.workspace);
+  ScoredMmaParams p{};
+  p.out = a.out;
+  p.q = a.query;
+  p.k_cache = a.key_cache;
+  p.v_cache = a.value_cache;
+  p.score_cache = a.score_cache;
+  p.block_tables = a.block_tables;
+  p.context_lens = a.context_lens;
+  p.k_scale = a.k_scale;
+  p.v_scale = a.v_scale;
+  p.ws_o = reinterpret_cast<float *>(ws + l.off_o);
+  p.ws_ml = reinterpret_cast<float2 *>(ws + l.off_ml);
+  p.ws_x = reinterpret_cast<float *>(ws + l.off_x);
+  p.counters = reinterpret_cast<uint32_t *>(ws + l.off_counters);
+  p.q_token_stride = a.q_token_stride;
+  p.num_blocks = a.num_blocks;
+  p.x_stride = l.x_stride;
+  p.num_heads = a.num_heads;
+  p.num_kv_heads = a.num_kv_heads;
+  p.group = a.num_heads / a.num_kv_heads;
+  p.query_len = a.query_len;
+  p.rows = a.query_len * p.group;
+  p.scored_rows = a.score_rows * p.group;
+  p.row_tiles = kDup ? 1 : (p.rows + 8 * NRT - 1) / (8 * NRT);
+  p.cols = a.max_num_blocks_per_seq;
+  p.max_context = a.max_context_len;
+  p.pages_per_split = l.pages_per_split;
+  p.max_splits = l.max_splits;
+  p.fused = a.max_context_len <= kMmaFusedContext && (int64_t)a.num_seqs * a.num_kv_heads <= kMaxCounters;
+  p.scale = a.scale;
+  p.softcap = a.softcapping;
+  p.decay = a.decay;
+  auto kern = scored_mma_kernel<T, TC, BS, NRT, kDup, kNST, kMinB>;
+  static std::atomic<uint64_t> attr_done{0};
+  if (!ensure_smem_attr(kern, C::kSmemBytes, attr_done)) return VASR_PA_ELAUNCH;
+  const dim3 grid((unsigned)l.max_splits, (unsigned)(a.num_kv_heads * p.row_tiles), (unsigned)a.num_seqs);
+  kern<<<grid, kScoredThreads, C::kSmemBytes, s>>>(p);
+  if (!p.fused) {
+    const int merge = (p.rows + 3) / 4;
+    const int chunks = (a.max_context_len + kJoinTokens - 1) / kJoinTokens;
+    scored_join_kernel<T><<<dim3((unsigned)(merge + chunks), (unsigned)a.num_kv_heads, (unsigned)a.num_seqs),
+                            kScoredThreads, 0, s>>>(p, BS, merge);
+  }
+  return cudaPeekAtLastError() == cudaSuccess ? VASR_PA_OK : VASR_PA_ELAUNCH;
+}
+
+template <typename T, typename TC, int BS>
+int launch_mma_bs(const ScoredArgs &a, cudaStream_t s) {
+  const int rows = a.query_len * (a.num_heads / a.num_kv_heads);
+  if (rows <= 4) return launch_mma_rows<T, TC, BS, 1, true>(a, s);
+  if (rows <= 8) return launch_mma_rows<T, TC, BS, 1, false>(a, s);
+  return launch_mma_rows<T, TC, BS, 2, false>(a, s);
+}
+
 template <typename T>
 int launch_scored_c(const ScoredArgs &a, cudaStream_t s) {
+  if constexpr (!std::is_same<T, float>::value) {
+    if (takes_mma(a)) {
+      if (a.cache_dtype == VASR_PA_FP8_E4M3)
+        return a.block_size == 16 ? launch_mma_bs<T, __nv_fp8_e4m3, 16>(a, s) : launch_mma_bs<T, __nv_fp8_e4m3, 32>(a, s);
+      switch (a.block_size) {
+        case 8: return launch_mma_bs<T, T, 8>(a, s);
+        case 16: return launch_mma_bs<T, T, 16>(a, s);
+        default: return launch_mma_bs<T, T, 32>(a, s);
+      }
+    }
+  }
   if (a.cache_dtype == VASR_PA_FP8_E4M3) return launch_scored_t<T, __nv_fp8_e4m3>(a, s);
   return launch_scored_t<T, T>(a, s);
 }
@@ -220,8 +336,12 @@ int launch_scored_c(const ScoredArgs &a, cudaStream_t s) {
 
 size_t scored_workspace_bytes(int num_seqs, int query_len, int score_rows, int num_heads, int num_kv_heads,
                               int head_dim, int block_size, int max_context_len) {
-  (void)block_size;
-  return layout(num_seqs, query_len, score_rows, num_heads, num_kv_heads, head_dim, max_context_len).total;
+  const size_t mma =
+      head_dim == kScoredDim
+          ? mma_layout(num_seqs, query_len, score_rows, num_heads, num_kv_heads, block_size, max_context_len).total
+          : 0;
+  const size_t other = layout(num_seqs, query_len, score_rows, num_heads, head_dim, max_context_len).total;
+  return mma > other ? mma : other;
 }
 
 int launch_scored(const ScoredArgs &a, cudaStream_t s) {

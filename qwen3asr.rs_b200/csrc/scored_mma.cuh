@@ -1,0 +1,601 @@
+// scored_mma.cuh — scored decode attention on the tensor cores (mma.sync
+// m16n8k16, f32 accumulate) for 16-bit queries over 16-bit or fp8 pages,
+// head_dim 128.
+//
+// A CTA takes one split of one (sequence, kv head)'s context and 8 or 16 rows,
+// row r = i * group + g for window row i and query head g of the kv head. Its
+// pages stream through a ring of shared-memory stages by bulk copies; stage s
+// belongs to warp s % 4. Per 16 tokens a warp computes
+//   S[16 rows x 16] = Q K^T     A = Q, B = K by ldmatrix from the page layout
+//   O^T[128 x rows] += V^T P^T  A = V^T by ldmatrix, B = S's own fragments
+// and leaves the rows' raw scores x (log2 domain) in the workspace; the
+// weights follow once the row's maximum and sum over all splits are known.
+//
+// Up to 4 rows (kDup: one token, group <= 4) P^T has columns to spare: A holds
+// every query row twice, so the score fragments of rows r and r + 4 are equal,
+// and row r's P goes into the product rounded to the operand type while row
+// r + 4 carries what that rounding left. O then has P's full f32 precision up
+// to 2^-16, for no further MMA; with more rows P is rounded to the operand
+// type (the output has that rounding anyway).
+//
+// Tokens that only some rows of a window see (the last query_len - 1) stay
+// out of the P V product: a masked row would multiply their V by zero, and a
+// NaN or infinite V would then reach a row that does not see it. They are
+// added one by one in f32, row by row.
+//
+// fp8 pages: the products run in f16 (every E4M3 value is exact in f16), with
+// each query row scaled by a power of two to the top of f16's range, so that
+// bf16 rows of any magnitude keep their bits. The reduction index is permuted
+// as in decode_mma.cuh, so that one ldmatrix row of 16 bytes feeds a k-step.
+#pragma once
+
+#include "decode_mma.cuh"
+
+namespace vasr {
+
+constexpr int kScoredDim = 128;
+constexpr int kScoredMaxRows = 128;       // rows of one (sequence, kv head)
+constexpr int kScoredMaxPages = 64;       // pages of one split
+constexpr int kScoredThreads = 128;
+
+struct ScoredMmaParams {
+  void *out;
+  const void *q;
+  const void *k_cache;
+  const void *v_cache;
+  float *score_cache;
+  const uint32_t *block_tables;
+  const uint32_t *context_lens;
+  const float *k_scale;
+  const float *v_scale;
+  float *ws_o;         // [(b * Hkv + kvh) * max_splits + split][rows][D]
+  float2 *ws_ml;       // [..same..][rows]  (m in log2 units, l)
+  float *ws_x;         // [(b * Hkv + kvh) * scored_rows + r][x_stride]
+  uint32_t *counters;  // [b * Hkv + kvh]
+  int64_t q_token_stride;
+  int64_t num_blocks;
+  int64_t x_stride;
+  int num_heads;
+  int num_kv_heads;
+  int group;
+  int query_len;
+  int rows;            // query_len * group
+  int scored_rows;     // score_rows * group
+  int row_tiles;
+  int cols;
+  int max_context;
+  int pages_per_split;
+  int max_splits;
+  int fused;           // the last CTA of a (sequence, kv head) finishes it
+  float scale;
+  float softcap;
+  float decay;
+};
+
+// The context length a kernel works with; too long a one is cut and recorded.
+__device__ __forceinline__ int scored_context(const ScoredMmaParams &p, int b, int bs, bool report) {
+  int64_t n = p.context_lens[b];
+  const int64_t cap = min((int64_t)p.cols * bs, (int64_t)p.max_context);
+  if (n > cap) {
+    if (report) raise_device_error(VASR_PA_DERR_CTX_RANGE);
+    n = cap;
+  }
+  return (int)n;
+}
+
+__device__ __forceinline__ int scored_splits(int n, int pages_per_split, int bs) {
+  const int per = pages_per_split * bs;
+  return (n + per - 1) / per;
+}
+
+// (m, 1 / l) of rows [0, count) over the splits, into shared memory. A row
+// that saw nothing gets (0, 0): its raw scores are -inf and weigh 0.
+__device__ __forceinline__ void scored_final_rows(const ScoredMmaParams &p, int64_t pair, int n_splits, int count,
+                                                  float2 *fin) {
+  for (int r = threadIdx.x; r < count; r += kScoredThreads) {
+    const float2 *ml = p.ws_ml + pair * p.max_splits * p.rows + r;
+    float m = -INFINITY, l = 0.f;
+    for (int s = 0; s < n_splits; ++s) m = fmaxf(m, __ldcg(&ml[(int64_t)s * p.rows].x));
+    for (int s = 0; s < n_splits; ++s) {
+      const float2 v = __ldcg(&ml[(int64_t)s * p.rows]);
+      if (v.y != 0.f) l = fmaf(v.y, exp2f(v.x - m), l);
+    }
+    fin[r] = l != 0.f ? make_float2(m, 1.f / l) : make_float2(0.f, 0.f);
+  }
+}
+
+// Rows [r0, r1) of the output from the splits' partials.
+template <typename T>
+__device__ __forceinline__ void scored_merge_rows(const ScoredMmaParams &p, int b, int kvh, int n_splits, int r0, int r1,
+                                                  const float2 *fin, float v_mul) {
+  constexpr int D = kScoredDim;
+  const int64_t slot0 = ((int64_t)b * p.num_kv_heads + kvh) * p.max_splits;
+  for (int e = threadIdx.x; e < (r1 - r0) * (D / 4); e += kScoredThreads) {
+    const int r = r0 + e / (D / 4), d = e % (D / 4) * 4;
+    const float2 f = fin[r];
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < n_splits; ++s) {
+      const int64_t at = (slot0 + s) * p.rows + r;
+      const float2 ml = __ldcg(&p.ws_ml[at]);
+      if (ml.y == 0.f) continue;
+      const float w = exp2f(ml.x - f.x);
+      const float4 v = __ldcg(reinterpret_cast<const float4 *>(p.ws_o + at * D + d));
+      o.x = fmaf(v.x, w, o.x);
+      o.y = fmaf(v.y, w, o.y);
+      o.z = fmaf(v.z, w, o.z);
+      o.w = fmaf(v.w, w, o.w);
+    }
+    const float mul = f.y * v_mul;
+    T *out = static_cast<T *>(p.out) +
+             (((int64_t)b * p.query_len + r / p.group) * p.num_heads + kvh * p.group + r % p.group) * D + d;
+    out[0] = Elem<T>::from_f32(o.x * mul);
+    out[1] = Elem<T>::from_f32(o.y * mul);
+    out[2] = Elem<T>::from_f32(o.z * mul);
+    out[3] = Elem<T>::from_f32(o.w * mul);
+  }
+}
+
+// score <- decay score + sum of the scored rows' weights, tokens [j0, j1), 4
+// a thread (page rows hold a multiple of 8 tokens).
+__device__ __forceinline__ void scored_add_weights(const ScoredMmaParams &p, int b, int kvh, int bs, int j0, int j1,
+                                                   const float2 *fin) {
+  const float *x = p.ws_x + ((int64_t)b * p.num_kv_heads + kvh) * p.scored_rows * p.x_stride;
+  const uint32_t *table = p.block_tables + (int64_t)b * p.cols;
+  for (int j = j0 + threadIdx.x * 4; j < j1; j += kScoredThreads * 4) {
+    const uint32_t id = __ldg(table + j / bs);
+    if ((int64_t)id >= p.num_blocks) continue;  // recorded where the page was read
+    float4 *at = reinterpret_cast<float4 *>(p.score_cache + ((int64_t)id * p.num_kv_heads + kvh) * bs + j % bs);
+    const float4 old = *at;
+    float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int r = 0; r < p.scored_rows; ++r) {
+      const float2 f = fin[r];
+      const float4 v = __ldcg(reinterpret_cast<const float4 *>(x + r * p.x_stride + j));
+      w.x = fmaf(exp2f(v.x - f.x), f.y, w.x);
+      w.y = fmaf(exp2f(v.y - f.x), f.y, w.y);
+      w.z = fmaf(exp2f(v.z - f.x), f.y, w.z);
+      w.w = fmaf(exp2f(v.w - f.x), f.y, w.w);
+    }
+    const int left = j1 - j;  // places past the context keep their bits
+    float4 s = old;
+    s.x = fmaf(p.decay, old.x, w.x);
+    if (left > 1) s.y = fmaf(p.decay, old.y, w.y);
+    if (left > 2) s.z = fmaf(p.decay, old.z, w.z);
+    if (left > 3) s.w = fmaf(p.decay, old.w, w.w);
+    *at = s;
+  }
+}
+
+template <typename TC, int BS, int NST>
+struct ScoredCfg {
+  static constexpr int D = kScoredDim;
+  static constexpr int kWarps = kScoredThreads / 32;
+  static constexpr int kSP = BS < 16 ? 16 / BS : 1;  // pages per stage
+  static constexpr int kST = kSP * BS;               // tokens per stage
+  static constexpr int kTiles = kST / 16;
+  static constexpr int kPB = D * BS * (int)sizeof(TC);
+  static constexpr int kNST = NST;
+  static constexpr int kOffK = 0;
+  static constexpr int kOffV = NST * kSP * kPB;
+  static constexpr int kOffBlk = 2 * NST * kSP * kPB;
+  static constexpr int kOffBar = kOffBlk + kScoredMaxPages * 4;
+  static constexpr int kOffFin = kOffBar + NST * 8;                     // float2 [kScoredMaxRows]
+  static constexpr int kOffML = kOffFin + kScoredMaxRows * 8;           // float2 [warps][16]
+  static constexpr int kOffFlag = kOffML + kWarps * 16 * 8;
+  static constexpr int kSmemBytes = kOffFlag + 16;
+  static_assert(NST % kWarps == 0, "stages split evenly over the warps");
+  static_assert(kWarps * 16 * D * 4 <= kOffBlk, "the warps' O fits the drained ring");
+};
+
+template <typename T, typename TC, int BS, int NRT, bool kDup, int NST, int MINB>
+__global__ void __launch_bounds__(kScoredThreads, MINB) scored_mma_kernel(const ScoredMmaParams p) {
+  using C = ScoredCfg<TC, BS, NST>;
+  constexpr bool kFp8 = std::is_same<TC, __nv_fp8_e4m3>::value;
+  using TM = typename std::conditional<kFp8, __half, T>::type;  // MMA operand type
+  constexpr int D = C::D, kKS = D / 16, kRows = kDup ? 4 : 8 * NRT;
+  constexpr float kRescale = 8.f;  // the running maximum moves when a tile's exceeds it by 2^8
+  static_assert(!kDup || NRT == 1, "doubled rows fill one tile of 8");
+  extern __shared__ __align__(128) unsigned char smem[];
+  const uint32_t s_base = smem_addr(smem);
+  const int split = blockIdx.x, kvh = blockIdx.y / p.row_tiles, tile = blockIdx.y % p.row_tiles, b = blockIdx.z;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, grp = lane >> 2, tig = lane & 3;
+  if (tid < NST) mbar_init(s_base + C::kOffBar + tid * 8, 1);
+  if (tid == 0) mbar_fence_init();
+
+  const int n = scored_context(p, b, BS, split == 0 && tid == 0 && blockIdx.y == 0);
+  const int n_splits = scored_splits(n, p.pages_per_split, BS);
+  const int row0 = tile * kRows;
+  const float v_mul = p.v_scale ? __ldg(p.v_scale) : 1.f;
+  if (n == 0 && split == 0) {  // nothing cached: zeros
+    for (int e = tid; e < kRows * D; e += kScoredThreads) {
+      const int r = row0 + e / D;
+      if (r < p.rows)
+        static_cast<T *>(p.out)[(((int64_t)b * p.query_len + r / p.group) * p.num_heads + kvh * p.group + r % p.group) * D +
+                                e % D] = Elem<T>::from_f32(0.f);
+    }
+  }
+  if (split >= n_splits) return;
+  const int seq_pages = (n + BS - 1) / BS;
+  const int per = (seq_pages + n_splits - 1) / n_splits;  // pages shared evenly by the splits
+  const int page0 = split * per, tok0 = page0 * BS;
+  const int tok1 = min(n, tok0 + per * BS);
+  const int n_pages = max(0, (tok1 - tok0 + BS - 1) / BS);
+  const int n_units = (n_pages + C::kSP - 1) / C::kSP;
+  uint32_t *blk = reinterpret_cast<uint32_t *>(smem + C::kOffBlk);
+  if (tid < n_pages) {
+    uint32_t id = __ldg(p.block_tables + (int64_t)b * p.cols + page0 + tid);
+    if ((int64_t)id >= p.num_blocks) {
+      raise_device_error(VASR_PA_DERR_BLOCK_RANGE);
+      id = 0;
+    }
+    blk[tid] = id;
+  }
+  __syncthreads();
+
+  const TC *kc = static_cast<const TC *>(p.k_cache);
+  const TC *vc = static_cast<const TC *>(p.v_cache);
+  auto issue_unit = [&](int u) {
+    const int s = u % NST, pg0 = u * C::kSP, np = min(C::kSP, n_pages - pg0);
+    const uint32_t bar = s_base + C::kOffBar + s * 8;
+    mbar_arrive_expect_tx(bar, (uint32_t)(2 * np * C::kPB));
+    for (int i = 0; i < np; ++i) {
+      const int64_t off = ((int64_t)blk[pg0 + i] * p.num_kv_heads + kvh) * (D * BS);
+      bulk_g2s(s_base + C::kOffK + (s * C::kSP + i) * C::kPB, kc + off, C::kPB, bar);
+      bulk_g2s(s_base + C::kOffV + (s * C::kSP + i) * C::kPB, vc + off, C::kPB, bar);
+    }
+  };
+  if (lane == 0)
+    for (int u = warp; u < min(NST, n_units); u += C::kWarps) issue_unit(u);
+
+  // ---- query fragments: rows grp (and grp + 8) of this tile; row[t] = its row or -1
+  uint32_t qa[kKS][2 * NRT];
+  float c_log2[NRT];
+  int row[NRT];
+  const float k_mul = p.k_scale ? p.scale * __ldg(p.k_scale) : p.scale;
+#pragma unroll
+  for (int t = 0; t < NRT; ++t) {
+    const int r = row0 + (kDup ? (grp & 3) : grp + 8 * t);
+    row[t] = r < p.rows ? r : -1;
+    const int rr = r < p.rows ? r : 0;
+    const T *qp = static_cast<const T *>(p.q) + ((int64_t)b * p.query_len + rr / p.group) * p.q_token_stride +
+                  (int64_t)(kvh * p.group + rr % p.group) * D;
+    c_log2[t] = k_mul;
+    if constexpr (kFp8) {  // lane tig: dims 4 tig .. 4 tig + 3 of every k-step
+      float big = 0.f;
+      for (int ks = 0; ks < kKS; ++ks)
+        for (int e = 0; e < 4; ++e) big = fmaxf(big, fabsf(Elem<T>::to_f32(qp[ks * 16 + tig * 4 + e])));
+      big = warp_max_xor(big, 4);
+      // the row's largest value in [2^14, 2^15); exponents that would leave f32's range are cut
+      const int ex = min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 127);
+      const float up = __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
+      c_log2[t] *= __uint_as_float((uint32_t)(127 - 14 + ex) << 23);
+#pragma unroll
+      for (int ks = 0; ks < kKS; ++ks) {
+        const T *q4 = qp + ks * 16 + tig * 4;
+        qa[ks][2 * t] = dec_pack2<__half>(Elem<T>::to_f32(q4[0]) * up, Elem<T>::to_f32(q4[1]) * up);
+        qa[ks][2 * t + 1] = dec_pack2<__half>(Elem<T>::to_f32(q4[2]) * up, Elem<T>::to_f32(q4[3]) * up);
+      }
+    } else {
+#pragma unroll
+      for (int ks = 0; ks < kKS; ++ks) {
+        qa[ks][2 * t] = __ldg(reinterpret_cast<const uint32_t *>(qp + ks * 16 + tig * 2));
+        qa[ks][2 * t + 1] = __ldg(reinterpret_cast<const uint32_t *>(qp + ks * 16 + 8 + tig * 2));
+      }
+    }
+    if (row[t] < 0) {
+#pragma unroll
+      for (int ks = 0; ks < kKS; ++ks) qa[ks][2 * t] = qa[ks][2 * t + 1] = 0u;
+    }
+  }
+  const bool use_softcap = p.softcap != 1.f;
+  // row i of the window sees tokens below n - query_len + 1 + i; all rows those below n_all
+  const int n_all = n - p.query_len + 1;
+  int seen[NRT];
+  float *xrow[NRT];
+#pragma unroll
+  for (int t = 0; t < NRT; ++t) {
+    seen[t] = row[t] < 0 ? 0 : n_all + row[t] / p.group - tok0;
+    xrow[t] = nullptr;
+    if (row[t] >= 0 && row[t] < p.scored_rows && !(kDup && grp >= 4))
+      xrow[t] = p.ws_x + (((int64_t)b * p.num_kv_heads + kvh) * p.scored_rows + row[t]) * p.x_stride + tok0;
+    if (!use_softcap) c_log2[t] *= kLog2e;
+  }
+
+  float o[NRT][D / 16][4];
+  float m_used[NRT], l_part[NRT];
+#pragma unroll
+  for (int t = 0; t < NRT; ++t) {
+    m_used[t] = -INFINITY;
+    l_part[t] = 0.f;
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) o[t][j][0] = o[t][j][1] = o[t][j][2] = o[t][j][3] = 0.f;
+  }
+  bool aborted = false;
+  int u_abort = 0;
+  for (int u = warp; u < n_units; u += C::kWarps) {
+    const int s = u % NST;
+    if (!mbar_wait_bounded(s_base + C::kOffBar + s * 8, (uint32_t)((u / NST) & 1))) {
+      aborted = true;
+      u_abort = u;
+      break;
+    }
+    const uint32_t sk = s_base + C::kOffK + s * C::kSP * C::kPB;
+    const uint32_t sv = s_base + C::kOffV + s * C::kSP * C::kPB;
+    const int unit0 = u * C::kST;              // first token, relative to tok0
+    const int valid = tok1 - tok0 - unit0;     // cached tokens of the stage
+#pragma unroll
+    for (int ti = 0; ti < C::kTiles; ++ti) {
+      const int t0 = ti * 16;
+      if (t0 >= valid) break;
+      // ---- S = Q K^T, two 8-token n-tiles
+      float sacc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      if constexpr (kFp8) {
+        const int r = lane & 7;
+        const int ktok = t0 + 4 * (r >> 1) + 2 * ((lane >> 3) & 1) + (r & 1);
+        const uint32_t krow = sk + (ktok / BS) * C::kPB + ((lane >> 4) * BS + ktok % BS) * 16;
+#pragma unroll
+        for (int kp = 0; kp < kKS / 2; ++kp) {
+          uint32_t f[4];
+          dec_ldmatrix_x4(krow + kp * 2 * (BS * 16), f[0], f[1], f[2], f[3]);
+#pragma unroll
+          for (int q2 = 0; q2 < 4; ++q2) {
+            const int ks = 2 * kp + (q2 >> 1);
+            dec_mma<TM>(sacc[q2 & 1], qa[ks][0], NRT > 1 ? qa[ks][2 * NRT - 2] : 0u, qa[ks][1],
+                        NRT > 1 ? qa[ks][2 * NRT - 1] : 0u, fp8x2_to_h2(f[q2]), fp8x2_to_h2(f[q2] >> 16));
+          }
+        }
+      } else {
+        const int ktok = t0 + (lane & 7) + (lane >> 4) * 8;
+        const uint32_t krow = sk + (ktok / BS) * C::kPB + (ktok % BS) * 16 + ((lane >> 3) & 1) * (BS * 16);
+#pragma unroll
+        for (int ks = 0; ks < kKS; ++ks) {
+          uint32_t b0, b1, b2, b3;
+          dec_ldmatrix_x4(krow + ks * 2 * (BS * 16), b0, b1, b2, b3);
+          const uint32_t a1 = NRT > 1 ? qa[ks][2 * NRT - 2] : 0u, a3 = NRT > 1 ? qa[ks][2 * NRT - 1] : 0u;
+          dec_mma<TM>(sacc[0], qa[ks][0], a1, qa[ks][1], a3, b0, b1);
+          dec_mma<TM>(sacc[1], qa[ks][0], a1, qa[ks][1], a3, b2, b3);
+        }
+      }
+      // ---- raw scores of the lane's rows, tokens tok(n, e) of the tile
+      auto tok = [&](int nn, int e) { return kFp8 ? t0 + 4 * tig + 2 * nn + e : t0 + nn * 8 + tig * 2 + e; };
+      float pv[NRT][4];
+      uint32_t pa[NRT][2];
+#pragma unroll
+      for (int t = 0; t < NRT; ++t) {
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float v = sacc[e >> 1][2 * t + (e & 1)] * c_log2[t];
+          if (use_softcap) v = p.softcap * tanhf(v / p.softcap) * kLog2e;
+          const int j = tok(e >> 1, e & 1);
+          x[e] = j < valid && unit0 + j < seen[t] ? v : -INFINITY;
+        }
+        if (xrow[t]) {
+          if (tok(0, 0) < valid) *reinterpret_cast<float2 *>(xrow[t] + unit0 + tok(0, 0)) = make_float2(x[0], x[1]);
+          if (tok(1, 0) < valid) *reinterpret_cast<float2 *>(xrow[t] + unit0 + tok(1, 0)) = make_float2(x[2], x[3]);
+        }
+        float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        if (__any_sync(0xffffffffu, mx > m_used[t] + kRescale)) {
+          const float m_new = fmaxf(m_used[t], mx);
+          const float alpha = m_used[t] == -INFINITY ? 0.f : exp2f(m_used[t] - m_new);
+          m_used[t] = m_new;
+          l_part[t] *= alpha;
+          // O^T's columns 2 tig, 2 tig + 1 are rows whose alphas live in lanes 8 tig, 8 tig + 4
+          const float a0 = __shfl_sync(0xffffffffu, alpha, 8 * tig), a1 = __shfl_sync(0xffffffffu, alpha, 8 * tig + 4);
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j) {
+            o[t][j][0] *= a0;
+            o[t][j][1] *= a1;
+            o[t][j][2] *= a0;
+            o[t][j][3] *= a1;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          pv[t][e] = x[e] == -INFINITY ? 0.f : exp2f(x[e] - (m_used[t] == -INFINITY ? 0.f : m_used[t]));
+          l_part[t] += pv[t][e];
+        }
+#pragma unroll
+        for (int nn = 0; nn < 2; ++nn) {
+          pa[t][nn] = dec_pack2<TM>(pv[t][2 * nn], pv[t][2 * nn + 1]);
+          if constexpr (kDup) {  // rows 4..7: what the rounding of rows 0..3 left
+            const TM *h = reinterpret_cast<const TM *>(&pa[t][nn]);
+            const uint32_t rest = dec_pack2<TM>(pv[t][2 * nn] - Elem<TM>::to_f32(h[0]),
+                                                pv[t][2 * nn + 1] - Elem<TM>::to_f32(h[1]));
+            if (grp >= 4) pa[t][nn] = rest;
+          }
+        }
+      }
+      // ---- O^T += V^T P^T over the tokens that every row sees
+      const int whole = min(valid, n_all - tok0 - unit0);  // tokens of the stage below n_all
+      const bool tail = t0 + 16 > whole;
+      if constexpr (kFp8) {
+        const int vd = (lane >> 3) * 8 + (lane & 7);
+        const uint32_t vrow = sv + (t0 / BS) * C::kPB + vd * BS + t0 % BS;
+        const int tk = t0 + 4 * tig;
+        const uint32_t mlo = (tk < whole ? 0xffffu : 0u) | (tk + 1 < whole ? 0xffff0000u : 0u);
+        const uint32_t mhi = (tk + 2 < whole ? 0xffffu : 0u) | (tk + 3 < whole ? 0xffff0000u : 0u);
+#pragma unroll
+        for (int dq = 0; dq < D / 32; ++dq) {
+          uint32_t r[4];
+          dec_ldmatrix_x4(vrow + dq * 32 * BS, r[0], r[1], r[2], r[3]);
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            uint32_t a0 = fp8x2_to_h2(r[2 * hf]), a2 = fp8x2_to_h2(r[2 * hf] >> 16);
+            uint32_t a1 = fp8x2_to_h2(r[2 * hf + 1]), a3 = fp8x2_to_h2(r[2 * hf + 1] >> 16);
+            if (tail) {
+              a0 &= mlo;
+              a1 &= mlo;
+              a2 &= mhi;
+              a3 &= mhi;
+            }
+#pragma unroll
+            for (int t = 0; t < NRT; ++t) dec_mma<TM>(o[t][dq * 2 + hf], a0, a1, a2, a3, pa[t][0], pa[t][1]);
+          }
+        }
+      } else {
+        const int vd = (lane & 7) + (lane >> 4) * 8;
+        const int vtok = t0 + ((lane >> 3) & 1) * 8;
+        const uint32_t vrow = sv + (vtok / BS) * C::kPB + (vd * BS + vtok % BS) * 2;
+        const int tk = t0 + tig * 2;
+        const uint32_t m0 = (tk < whole ? 0xffffu : 0u) | (tk + 1 < whole ? 0xffff0000u : 0u);
+        const uint32_t m1 = (tk + 8 < whole ? 0xffffu : 0u) | (tk + 9 < whole ? 0xffff0000u : 0u);
+#pragma unroll
+        for (int dp = 0; dp < D / 16; ++dp) {
+          uint32_t b0, b1, b2, b3;
+          dec_ldmatrix_x4(vrow + dp * 16 * BS * 2, b0, b1, b2, b3);
+          if (tail) {
+            b0 &= m0;
+            b2 &= m0;
+            b1 &= m1;
+            b3 &= m1;
+          }
+#pragma unroll
+          for (int t = 0; t < NRT; ++t) dec_mma<TM>(o[t][dp], b0, b2, b1, b3, pa[t][0], pa[t][1]);
+        }
+      }
+      // ---- tokens that only some rows see, one by one
+      if (tail && whole < valid) {
+        const unsigned char *vp = smem + C::kOffV + s * C::kSP * C::kPB;
+        for (int j = max(t0, whole); j < min(t0 + 16, valid); ++j) {
+          const int jt = j - t0;
+          const int src = kFp8 ? jt >> 2 : (jt & 7) >> 1;                 // tig of the token's lane
+          const int at = kFp8 ? jt & 3 : 2 * (jt >> 3) + (jt & 1);        // its place there
+#pragma unroll
+          for (int t = 0; t < NRT; ++t) {
+            float w[2];
+            bool sees[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {  // the lane's columns of O^T: rows 2 tig + e
+              const int from = (2 * tig + e) * 4 + src;
+              float v0 = __shfl_sync(0xffffffffu, pv[t][0], from), v1 = __shfl_sync(0xffffffffu, pv[t][1], from);
+              float v2 = __shfl_sync(0xffffffffu, pv[t][2], from), v3 = __shfl_sync(0xffffffffu, pv[t][3], from);
+              w[e] = at == 0 ? v0 : at == 1 ? v1 : at == 2 ? v2 : v3;
+              sees[e] = unit0 + j < __shfl_sync(0xffffffffu, seen[t], (2 * tig + e) * 4);
+              if (kDup && tig >= 2) sees[e] = false;  // the doubled rows' columns
+            }
+#pragma unroll
+            for (int jd = 0; jd < D / 16; ++jd)
+#pragma unroll
+              for (int hf = 0; hf < 2; ++hf) {
+                const int d = jd * 16 + hf * 8 + grp;
+                const TC v = reinterpret_cast<const TC *>(vp + (j / BS) * C::kPB)[d * BS + j % BS];
+                if (sees[0]) o[t][jd][2 * hf] = fmaf(w[0], Elem<TC>::to_f32(v), o[t][jd][2 * hf]);
+                if (sees[1]) o[t][jd][2 * hf + 1] = fmaf(w[1], Elem<TC>::to_f32(v), o[t][jd][2 * hf + 1]);
+              }
+          }
+        }
+      }
+    }
+    __syncwarp();
+    const int nu = u + NST;
+    if (nu < n_units && lane == 0) {
+      fence_proxy_async_smem();
+      issue_unit(nu);
+    }
+  }
+  if (aborted) {  // the copies this warp has in flight land before the ring is reused
+    for (int v = u_abort; v < min(u_abort + NST, n_units); v += C::kWarps)
+      mbar_wait_bounded(s_base + C::kOffBar + (v % NST) * 8, (uint32_t)((v / NST) & 1));
+  }
+  __syncthreads();  // every stage is read: the ring becomes the warps' O
+
+  float *co = reinterpret_cast<float *>(smem);  // [warp][kRows][D]
+  float2 *cml = reinterpret_cast<float2 *>(smem + C::kOffML);  // [warp][16]
+#pragma unroll
+  for (int t = 0; t < NRT; ++t) {
+    float l = l_part[t];
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    if (tig == 0 && !(kDup && grp >= 4))
+      cml[warp * 16 + 8 * t + grp] = aborted ? make_float2(-INFINITY, 0.f) : make_float2(m_used[t], l);
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float v = o[t][j][e];
+        if constexpr (kDup) v += __shfl_xor_sync(0xffffffffu, v, 2);  // rows r and r + 4
+        const int r = 8 * t + 2 * tig + (e & 1), d = j * 16 + (e >> 1) * 8 + grp;
+        if (r < kRows) co[(warp * kRows + r) * D + d] = v;
+      }
+  }
+  __syncthreads();
+  const int64_t pair = (int64_t)b * p.num_kv_heads + kvh;
+  const bool alone = n_splits == 1 && p.row_tiles == 1 && p.fused;
+  float2 *fin = reinterpret_cast<float2 *>(smem + C::kOffFin);
+  const int rows_here = min(kRows, p.rows - row0);
+  for (int e = tid; e < rows_here * D; e += kScoredThreads) {
+    const int r = e / D, d = e % D;
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < C::kWarps; ++w) m = fmaxf(m, cml[w * 16 + r].x);
+    float l = 0.f, ov = 0.f;
+#pragma unroll
+    for (int w = 0; w < C::kWarps; ++w) {
+      const float2 ml = cml[w * 16 + r];
+      if (ml.y == 0.f) continue;
+      const float f = exp2f(ml.x - m);
+      l = fmaf(ml.y, f, l);
+      ov = fmaf(co[(w * kRows + r) * D + d], f, ov);
+    }
+    if (alone) {
+      const float inv = l != 0.f ? 1.f / l : 0.f;
+      if (d == 0) fin[r] = l != 0.f ? make_float2(m, inv) : make_float2(0.f, 0.f);
+      static_cast<T *>(p.out)[(((int64_t)b * p.query_len + r / p.group) * p.num_heads + kvh * p.group + r % p.group) * D +
+                              d] = Elem<T>::from_f32(ov * inv * v_mul);
+    } else {
+      const int64_t at = (pair * p.max_splits + split) * p.rows + row0 + r;
+      p.ws_o[at * D + d] = ov;
+      if (d == 0) p.ws_ml[at] = make_float2(m, l);
+    }
+  }
+  if (!p.fused) return;
+  if (!alone) {
+    // the last CTA of this (sequence, kv head) to get here finishes it
+    __threadfence();
+    __syncthreads();
+    uint32_t *flag = reinterpret_cast<uint32_t *>(smem + C::kOffFlag);
+    if (tid == 0) {
+      const uint32_t all = (uint32_t)(n_splits * p.row_tiles);
+      flag[0] = atomicAdd(p.counters + pair, 1u) == all - 1;
+      __threadfence();
+    }
+    __syncthreads();
+    if (!flag[0]) return;
+    if (tid == 0) p.counters[pair] = 0u;
+    scored_final_rows(p, pair, n_splits, p.rows, fin);
+    __syncthreads();
+    scored_merge_rows<T>(p, b, kvh, n_splits, 0, p.rows, fin, v_mul);
+  } else {
+    __syncthreads();  // fin, and this CTA's raw scores
+  }
+  scored_add_weights(p, b, kvh, BS, 0, n, fin);
+}
+
+// The end of every (sequence, kv head) as a launch of its own, for long
+// contexts: blocks [0, merge_blocks) join 4 rows each, the others add the
+// weights of kJoinTokens tokens each.
+constexpr int kJoinTokens = 1024;
+template <typename T>
+__global__ void __launch_bounds__(kScoredThreads) scored_join_kernel(const ScoredMmaParams p, int bs, int merge_blocks) {
+  __shared__ float2 fin[kScoredMaxRows];
+  pdl_wait();
+  const int kvh = blockIdx.y, b = blockIdx.z;
+  const int n = scored_context(p, b, bs, false);
+  const int n_splits = scored_splits(n, p.pages_per_split, bs);
+  const int64_t pair = (int64_t)b * p.num_kv_heads + kvh;
+  const bool merge = (int)blockIdx.x < merge_blocks;
+  const int j0 = ((int)blockIdx.x - merge_blocks) * kJoinTokens;
+  if (n == 0 || (!merge && j0 >= n)) return;
+  scored_final_rows(p, pair, n_splits, merge ? p.rows : p.scored_rows, fin);
+  __syncthreads();
+  if (merge) {
+    const int r0 = blockIdx.x * 4;
+    scored_merge_rows<T>(p, b, kvh, n_splits, r0, min(r0 + 4, p.rows), fin, p.v_scale ? __ldg(p.v_scale) : 1.f);
+  } else {
+    scored_add_weights(p, b, kvh, bs, j0, min(n, j0 + kJoinTokens), fin);
+  }
+}
+
+}  // namespace vasr
