@@ -269,6 +269,12 @@ struct VerifyArgs {
   int num_drafts;
   int64_t vocab;
   void *workspace;
+  // filled by launch_verify
+  int num_chunks;
+  int chunk_elems;
+  void *stats;
+  void *bests;
+  uint32_t *counters;
 };
 size_t verify_workspace_bytes(int num_seqs, int num_drafts, int64_t vocab);
 int launch_verify(const VerifyArgs &a, cudaStream_t s);

@@ -11,64 +11,46 @@
 // sum over the vocabulary, the comparison does not depend on the order of a
 // long f32 sum. T = 0: accept while x_i is the argmax of row i, then take row
 // n's argmax. Lowest index on equal values; NaN logits count as -inf.
+//
+// Two launches. The first gives every chunk of every row its maximum and its
+// sum of exp((x - max) / T) in one pass: a thread keeps its 32 logits in
+// registers between the maximum and the sum. The second, a programmatic
+// dependent of the first, has a CTA per chunk of a sequence's vocabulary: it
+// loads its noise and the drafts' logits early, joins the rows' chunks and
+// decides on its own copy (a few hundred bytes), runs the race over its chunk
+// of row n, and the last CTA of the sequence takes the winner. Only the row
+// that is drawn from is read twice, the second time from L2.
 #include "common.cuh"
 #include "launch.h"
 
 namespace vasr {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kPerThread = 32;  // logits a thread keeps in registers
+constexpr int kMaxThreads = 256;
 
-// What row i says: its maximum (and where), the sum of exp((x - max) / T).
-struct RowStat {
+// One chunk of a row: its maximum (and, for greedy rows, the first place of
+// it) and sum over the chunk of exp((x - max) / T).
+struct ChunkStat {
   float max;
   float sum;
   uint32_t arg;
   uint32_t pad;
 };
 
-template <typename T>
-__device__ __forceinline__ float load_logit(const T *row, int64_t v) {
-  const float x = Elem<T>::to_f32(row[v]);
-  return x == x ? x : -INFINITY;
-}
-
-__device__ __forceinline__ float load_prob(const void *row, int64_t v, int dtype) {
-  switch (dtype) {
-    case VASR_PA_BF16: return __bfloat162float(static_cast<const __nv_bfloat16 *>(row)[v]);
-    case VASR_PA_F16: return __half2float(static_cast<const __half *>(row)[v]);
-    default: return static_cast<const float *>(row)[v];
-  }
-}
-
 // (value, index): larger value first, then lower index.
 struct Best {
   float v;
   uint32_t i;
 };
+constexpr uint32_t kNone = 0xffffffffu;
 __device__ __forceinline__ Best better(Best x, Best y) {
   return (y.v > x.v || (y.v == x.v && y.i < x.i)) ? y : x;
 }
-__device__ __forceinline__ Best block_best(Best x) {
-  __shared__ Best part[kThreads / 32];
+__device__ __forceinline__ Best warp_best(Best x) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1)
     x = better(x, Best{__shfl_xor_sync(0xffffffffu, x.v, o), __shfl_xor_sync(0xffffffffu, x.i, o)});
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = x;
-  __syncthreads();
-  x = part[0];
-  for (int w = 1; w < kThreads / 32; ++w) x = better(x, part[w]);
-  __syncthreads();
-  return x;
-}
-__device__ __forceinline__ float block_sum(float x) {
-  __shared__ float part[kThreads / 32];
-  x = warp_sum_xor(x, 32);
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = x;
-  __syncthreads();
-  x = 0.f;
-  for (int w = 0; w < kThreads / 32; ++w) x += part[w];
-  __syncthreads();
   return x;
 }
 
@@ -78,100 +60,332 @@ __device__ __forceinline__ float temperature_of(const VerifyArgs &p, int b) {
 __device__ __forceinline__ int drafts_of(const VerifyArgs &p, int b) {
   return p.draft_lens ? min(max(p.draft_lens[b], 0), p.num_drafts) : p.num_drafts;
 }
-// exp((x - max) / T); the entries at an infinite maximum share the mass.
-__device__ __forceinline__ float weight_of(float x, float max, float inv_t) {
-  return x == max ? 1.f : expf((x - max) * inv_t);
+// exp((x - max) / T) with c = log2(e) / T; the entries at an infinite maximum
+// share the mass, and -inf weighs nothing.
+__device__ __forceinline__ float weight_of(float x, float max, float c) {
+  return x == max ? 1.f : exp2f((x - max) * c);
 }
 
+// A thread's elements of a chunk of a row: groups of 8, group tid + k threads
+// being its k-th whatever the type, so that rows of different types line up.
+// Vector loads where the group is 16-byte aligned and whole, else one by one
+// (what lies past the chunk reads as 0).
+constexpr int kGroup = 8;
+constexpr int kGroups = kPerThread / kGroup;
 template <typename T>
-__global__ void __launch_bounds__(kThreads) verify_rows_kernel(const VerifyArgs p) {
-  const int i = blockIdx.x, b = blockIdx.y;
+struct Held {
+  static constexpr int kVec = 16 / (int)sizeof(T);
+  static constexpr int kVecs = kGroup / kVec;
+  uint4 raw[kGroups][kVecs];
+  __device__ __forceinline__ void load(const T *row, int len, int tid, int threads) {
+    const bool aligned = reinterpret_cast<uintptr_t>(row) % 16 == 0;
+#pragma unroll
+    for (int k = 0; k < kGroups; ++k) {
+      const int j = (tid + k * threads) * kGroup;
+      if (aligned && j + kGroup <= len) {
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) raw[k][v] = __ldg(reinterpret_cast<const uint4 *>(row + j) + v);
+      } else {
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) {
+          T e[kVec];
+#pragma unroll
+          for (int i = 0; i < kVec; ++i) {
+            const int at = j + v * kVec + i;
+            e[i] = at < len ? row[at] : Elem<T>::from_f32(0.f);
+          }
+          raw[k][v] = *reinterpret_cast<const uint4 *>(e);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void group(int k, float (&out)[kGroup]) const {
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v) {
+      float f[kVec];
+      unpack_chunk<T>(raw[k][v], f);
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) out[v * kVec + i] = f[i];
+    }
+  }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kMaxThreads) verify_rows_kernel(const VerifyArgs p) {
+  pdl_launch_dependents();
+  const int chunk = blockIdx.x, i = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, threads = blockDim.x;
   if (i > drafts_of(p, b)) return;
-  const T *row = static_cast<const T *>(p.logits) + b * p.logits_seq_stride + i * p.logits_row_stride;
-  Best best{-INFINITY, 0xffffffffu};
-  for (int64_t v = threadIdx.x; v < p.vocab; v += kThreads) {
-    const float x = load_logit(row, v);
-    if (x > best.v) best = Best{x, (uint32_t)v};
-  }
-  best = block_best(best);
+  const int64_t lo = (int64_t)chunk * p.chunk_elems;
+  const int len = (int)min((int64_t)p.chunk_elems, p.vocab - lo);
+  const T *row = static_cast<const T *>(p.logits) + b * p.logits_seq_stride + i * p.logits_row_stride + lo;
+  Held<T> x;
+  x.load(row, len, tid, threads);
   const float t = temperature_of(p, b);
+  // f(logit, index) for the thread's elements; NaN counts as -inf
+  auto each = [&](auto f) {
+#pragma unroll
+    for (int k = 0; k < kGroups; ++k) {
+      const int j = (tid + k * threads) * kGroup;
+      float v[kGroup];
+      x.group(k, v);
+      if (j + kGroup <= len) {
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i) f(fmaxf(v[i], -INFINITY), j + i);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i)
+          if (j + i < len) f(fmaxf(v[i], -INFINITY), j + i);
+      }
+    }
+  };
+  float m = -INFINITY;
+  each([&](float v, int) { m = fmaxf(m, v); });
+  __shared__ float part[kMaxThreads / 32];
+  __shared__ uint32_t s_arg;
+  const int warps = threads >> 5;
+  m = warp_max_xor(m, 32);
+  if ((tid & 31) == 0) part[tid >> 5] = m;
+  if (tid == 0) s_arg = kNone;
+  __syncthreads();
+  for (int w = 0; w < warps; ++w) m = fmaxf(m, part[w]);
+  __syncthreads();
   float sum = 0.f;
-  if (t > 0.f && best.v > -INFINITY) {
-    const float inv_t = 1.f / t;
-    for (int64_t v = threadIdx.x; v < p.vocab; v += kThreads) sum += weight_of(load_logit(row, v), best.v, inv_t);
-    sum = block_sum(sum);
+  if (t > 0.f) {
+    const float c = kLog2e / t;
+    if (m > -INFINITY) each([&](float v, int) { sum += weight_of(v, m, c); });
+    sum = warp_sum_xor(sum, 32);
+    if ((tid & 31) == 0) part[tid >> 5] = sum;
+    __syncthreads();
+    sum = 0.f;
+    for (int w = 0; w < warps; ++w) sum += part[w];
+  } else {
+    uint32_t first = kNone;
+    each([&](float v, int j) {
+      if (v == m) first = min(first, (uint32_t)j);
+    });
+    if (first != kNone) atomicMin(&s_arg, first);
+    __syncthreads();
   }
-  if (threadIdx.x == 0)
-    static_cast<RowStat *>(p.workspace)[(int64_t)b * (p.num_drafts + 1) + i] =
-        RowStat{best.v, sum, best.v > -INFINITY ? best.i : 0u, 0u};
+  if (tid == 0) {
+    ChunkStat *out = static_cast<ChunkStat *>(p.stats);
+    out[((int64_t)b * (p.num_drafts + 1) + i) * p.num_chunks + chunk] =
+        ChunkStat{m, sum, s_arg != kNone ? (uint32_t)lo + s_arg : 0u, 0u};
+  }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) verify_emit_kernel(const VerifyArgs p) {
-  const int b = blockIdx.x;
+// A whole row from its chunks, by one warp.
+__device__ __forceinline__ ChunkStat join_chunks(const VerifyArgs &p, int64_t row, float t) {
+  const int lane = threadIdx.x & 31;
+  const ChunkStat *s = static_cast<const ChunkStat *>(p.stats) + row * p.num_chunks;
+  Best top{-INFINITY, kNone};
+  for (int c = lane; c < p.num_chunks; c += 32)
+    if (s[c].max > -INFINITY) top = better(top, Best{s[c].max, s[c].arg});
+  top = warp_best(top);
+  float sum = 0.f;
+  if (t > 0.f && top.v > -INFINITY) {
+    const float k = kLog2e / t;
+    for (int c = lane; c < p.num_chunks; c += 32)
+      if (s[c].sum != 0.f) sum = fmaf(s[c].sum, weight_of(s[c].max, top.v, k), sum);
+    sum = warp_sum_xor(sum, 32);
+  }
+  return ChunkStat{top.v, sum, top.i != kNone ? top.i : 0u, 0u};
+}
+
+template <typename T, typename TQ>
+__global__ void __launch_bounds__(kMaxThreads) verify_emit_kernel(const VerifyArgs p) {
+  extern __shared__ ChunkStat s_row[];  // [num_drafts + 1]
+  __shared__ int s_fail;
+  __shared__ Best part[kMaxThreads / 32];
+  __shared__ uint32_t s_last;
+  const int chunk = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, threads = blockDim.x;
+  const int warp = tid >> 5, lane = tid & 31, warps = threads >> 5;
   const int k = drafts_of(p, b);
   const float t = temperature_of(p, b);
-  const float inv_t = t > 0.f ? 1.f / t : 0.f;
-  const RowStat *stats = static_cast<const RowStat *>(p.workspace) + (int64_t)b * (p.num_drafts + 1);
   const T *rows = static_cast<const T *>(p.logits) + b * p.logits_seq_stride;
+  const TQ *probs = p.draft_probs ? static_cast<const TQ *>(p.draft_probs) + b * p.probs_seq_stride : nullptr;
   const int32_t *drafts = p.draft_tokens + (int64_t)b * p.num_drafts;
-  const unsigned char *probs = nullptr;
-  const int prob_size = p.probs_dtype == VASR_PA_F32 ? 4 : 2;
-  if (p.draft_probs) probs = static_cast<const unsigned char *>(p.draft_probs) + b * p.probs_seq_stride * prob_size;
-  int n = 0;
-  for (; n < k; ++n) {
-    const int32_t x = drafts[n];
-    const RowStat s = stats[n];
-    if (x < 0 || x >= p.vocab || !(s.max > -INFINITY)) break;
-    if (t > 0.f) {
-      const float px = weight_of(load_logit(rows + n * p.logits_row_stride, x), s.max, inv_t) / s.sum;
-      const float qx = probs ? load_prob(probs + n * p.probs_row_stride * prob_size, x, p.probs_dtype) : 1.f;
-      if (!(p.uniform[(int64_t)b * p.num_drafts + n] * qx < px)) break;
-    } else if ((uint32_t)x != s.arg) {
-      break;
+  const int64_t lo = (int64_t)chunk * p.chunk_elems;
+  const int len = (int)min((int64_t)p.chunk_elems, p.vocab - lo);
+  if (tid == 0) s_fail = k;
+  // inputs that the first launch does not write
+  Held<float> race;
+  if (t > 0.f) race.load(p.race + b * p.race_seq_stride + lo, len, tid, threads);
+  int32_t x0 = -1;
+  float logit0 = -INFINITY, q0 = 1.f, u0 = 0.f;
+  if (tid < k) {
+    x0 = drafts[tid];
+    if (x0 >= 0 && x0 < p.vocab) {
+      logit0 = fmaxf(Elem<T>::to_f32(rows[tid * p.logits_row_stride + x0]), -INFINITY);
+      if (probs) q0 = Elem<TQ>::to_f32(probs[tid * p.probs_row_stride + x0]);
     }
+    if (t > 0.f) u0 = p.uniform[(int64_t)b * p.num_drafts + tid];
   }
-  const RowStat s = stats[n];
+  pdl_wait();
+  for (int i = warp; i <= k; i += warps) {
+    const ChunkStat s = join_chunks(p, (int64_t)b * (p.num_drafts + 1) + i, t);
+    if (lane == 0) s_row[i] = s;
+  }
+  __syncthreads();
+  const float c = t > 0.f ? kLog2e / t : 0.f;
+  for (int i = tid; i < k; i += threads) {
+    int32_t x = x0;
+    float logit = logit0, q = q0, u = u0;
+    if (i != tid) {
+      x = drafts[i];
+      logit = -INFINITY;
+      q = 1.f;
+      u = t > 0.f ? p.uniform[(int64_t)b * p.num_drafts + i] : 0.f;
+      if (x >= 0 && x < p.vocab) {
+        logit = fmaxf(Elem<T>::to_f32(rows[i * p.logits_row_stride + x]), -INFINITY);
+        if (probs) q = Elem<TQ>::to_f32(probs[i * p.probs_row_stride + x]);
+      }
+    }
+    const ChunkStat s = s_row[i];
+    bool ok = x >= 0 && x < p.vocab && s.max > -INFINITY;
+    if (ok) ok = t > 0.f ? u * q < weight_of(logit, s.max, c) / s.sum : (uint32_t)x == s.arg;
+    if (!ok) atomicMin(&s_fail, i);
+  }
+  __syncthreads();
+  const int n = s_fail;
+  const ChunkStat s = s_row[n];
+  const T *row = rows + n * p.logits_row_stride;
+  const int64_t failed = n < k ? (int64_t)drafts[n] : -1;
+  const TQ *qrow = probs && n < k ? probs + n * p.probs_row_stride : nullptr;
+  const bool drawn = t > 0.f && s.max > -INFINITY;
   uint32_t next = s.arg;
-  if (t > 0.f && s.max > -INFINITY) {
-    const T *row = rows + n * p.logits_row_stride;
-    const float *race = p.race + b * p.race_seq_stride;
-    const int64_t failed = n < k ? (int64_t)drafts[n] : -1;
-    const unsigned char *q = probs && n < k ? probs + n * p.probs_row_stride * prob_size : nullptr;
-    Best rest{0.f, 0xffffffffu}, all{0.f, 0xffffffffu};  // only positive values win
-    for (int64_t v = threadIdx.x; v < p.vocab; v += kThreads) {
-      const float pv = weight_of(load_logit(row, v), s.max, inv_t) / s.sum;
-      float r = pv;
-      if (q) r = pv - load_prob(q, v, p.probs_dtype);
-      else if (v == failed) r = 0.f;
-      const float e = race[v];
-      const float a = r / e, c = pv / e;
-      if (r > 0.f && a > rest.v) rest = Best{a, (uint32_t)v};
-      if (pv > 0.f && c > all.v) all = Best{c, (uint32_t)v};
+  if (drawn) {
+    // ---- the race over this chunk; a quotient is taken only where it wins
+    Held<T> x;
+    x.load(row + lo, len, tid, threads);
+    Held<TQ> q;
+    if (qrow) q.load(qrow + lo, len, tid, threads);
+    const float inv = 1.f / s.sum;
+    Best best{-1.f, kNone};
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      const int j = (tid + g * threads) * kGroup;
+      float w[kGroup], e[kGroup], qv[kGroup];
+      x.group(g, w);
+      race.group(g, e);
+      if (qrow) q.group(g, qv);
+#pragma unroll
+      for (int i = 0; i < kGroup; ++i) {
+        float r = weight_of(fmaxf(w[i], -INFINITY), s.max, c) * inv;
+        if (qrow) r -= qv[i];
+        else if (lo + j + i == failed) r = 0.f;
+        if (j + i < len && r > 0.f && r > best.v * e[i]) {
+          const float a = r / e[i];
+          if (a > best.v) best = Best{a, (uint32_t)(lo + j + i)};
+        }
+      }
     }
-    rest = block_best(rest);
-    all = block_best(all);
-    if (all.i == 0xffffffffu) all.i = s.arg;  // no weight over its noise is positive
-    next = rest.i != 0xffffffffu ? rest.i : all.i;
+    best = warp_best(best);
+    if (lane == 0) part[warp] = best;
+    __syncthreads();
+    if (tid == 0) {
+      for (int w = 1; w < warps; ++w) best = better(best, part[w]);
+      Best *slots = static_cast<Best *>(p.bests) + (int64_t)b * p.num_chunks;
+      slots[chunk] = best;
+      __threadfence();
+      s_last = atomicAdd(p.counters + b, 1u) == (uint32_t)p.num_chunks - 1;
+      __threadfence();
+    }
+    __syncthreads();
+    if (!s_last) return;
+    // ---- the sequence's last CTA: the winner over all chunks
+    best = Best{-1.f, kNone};
+    const Best *slots = static_cast<const Best *>(p.bests) + (int64_t)b * p.num_chunks;
+    for (int i = tid; i < p.num_chunks; i += threads) best = better(best, Best{__ldcg(&slots[i].v), __ldcg(&slots[i].i)});
+    best = warp_best(best);
+    if (lane == 0) part[warp] = best;
+    __syncthreads();
+    best = part[0];
+    for (int w = 1; w < warps; ++w) best = better(best, part[w]);
+    if (best.i == kNone) {  // r is 0 everywhere (the drafter covers the target): draw from p
+      __syncthreads();
+      const float *noise = p.race + b * p.race_seq_stride;
+      for (int64_t v = tid; v < p.vocab; v += threads) {
+        const float pv = weight_of(fmaxf(Elem<T>::to_f32(row[v]), -INFINITY), s.max, c) * inv;
+        const float a = pv / noise[v];
+        if (pv > 0.f && a > best.v) best = Best{a, (uint32_t)v};
+      }
+      best = warp_best(best);
+      if (lane == 0) part[warp] = best;
+      __syncthreads();
+      best = part[0];
+      for (int w = 1; w < warps; ++w) best = better(best, part[w]);
+    }
+    next = best.i != kNone ? best.i : 0u;  // all noise NaN
+    if (tid == 0) p.counters[b] = 0u;
+  } else if (chunk != 0) {
+    return;
   }
-  if (threadIdx.x == 0) {
-    int32_t *out = p.out_tokens + (int64_t)b * (p.num_drafts + 1);
-    for (int i = 0; i <= p.num_drafts; ++i) out[i] = i < n ? drafts[i] : i == n ? (int32_t)next : -1;
-    p.num_accepted[b] = n;
-  }
+  int32_t *out = p.out_tokens + (int64_t)b * (p.num_drafts + 1);
+  for (int i = tid; i <= p.num_drafts; i += threads) out[i] = i < n ? drafts[i] : i == n ? (int32_t)next : -1;
+  if (tid == 0) p.num_accepted[b] = n;
+}
+
+// 8192 logits a chunk (256 threads); calls whose chunks would not fill the SMs
+// take chunks of 2048 (64 threads), which cost more CTAs per byte.
+int chunk_threads(int num_seqs, int num_drafts, int64_t vocab) {
+  const int64_t ctas = (int64_t)num_seqs * (num_drafts + 1) * ((vocab + 8191) / 8192);
+  return ctas >= 2 * 148 ? 256 : 64;
+}
+
+struct VerifyLayout {
+  int threads, num_chunks;
+  size_t off_stats, off_bests, total;
+};
+constexpr size_t kCounterBytes = 65536 * sizeof(uint32_t);  // one per sequence, left at zero
+VerifyLayout verify_layout(int num_seqs, int num_drafts, int64_t vocab) {
+  VerifyLayout l;
+  l.threads = chunk_threads(num_seqs, num_drafts, vocab);
+  const int64_t per = (int64_t)l.threads * kPerThread;
+  l.num_chunks = (int)((vocab + per - 1) / per);
+  l.off_stats = kCounterBytes;
+  l.off_bests = l.off_stats + (size_t)num_seqs * (num_drafts + 1) * l.num_chunks * sizeof(ChunkStat);
+  l.total = l.off_bests + (size_t)num_seqs * l.num_chunks * sizeof(Best);
+  return l;
+}
+
+template <typename T, typename TQ>
+int launch_verify_tq(VerifyArgs a, cudaStream_t s) {
+  const VerifyLayout l = verify_layout(a.num_seqs, a.num_drafts, a.vocab);
+  unsigned char *ws = static_cast<unsigned char *>(a.workspace);
+  a.counters = reinterpret_cast<uint32_t *>(ws);
+  a.stats = ws + l.off_stats;
+  a.bests = ws + l.off_bests;
+  a.num_chunks = l.num_chunks;
+  a.chunk_elems = l.threads * kPerThread;
+  verify_rows_kernel<T><<<dim3((unsigned)l.num_chunks, (unsigned)a.num_drafts + 1, (unsigned)a.num_seqs),
+                          (unsigned)l.threads, 0, s>>>(a);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)l.num_chunks, (unsigned)a.num_seqs);
+  cfg.blockDim = dim3((unsigned)l.threads);
+  cfg.dynamicSmemBytes = (size_t)(a.num_drafts + 1) * sizeof(ChunkStat);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, verify_emit_kernel<T, TQ>, a) == cudaSuccess ? VASR_PA_OK : VASR_PA_ELAUNCH;
 }
 
 template <typename T>
 int launch_verify_t(const VerifyArgs &a, cudaStream_t s) {
-  verify_rows_kernel<T><<<dim3((unsigned)a.num_drafts + 1, (unsigned)a.num_seqs), kThreads, 0, s>>>(a);
-  verify_emit_kernel<T><<<(unsigned)a.num_seqs, kThreads, 0, s>>>(a);
-  return cudaPeekAtLastError() == cudaSuccess ? VASR_PA_OK : VASR_PA_ELAUNCH;
+  if (!a.draft_probs) return launch_verify_tq<T, float>(a, s);
+  switch (a.probs_dtype) {
+    case VASR_PA_BF16: return launch_verify_tq<T, __nv_bfloat16>(a, s);
+    case VASR_PA_F16: return launch_verify_tq<T, __half>(a, s);
+    default: return launch_verify_tq<T, float>(a, s);
+  }
 }
 
 }  // namespace
 
-size_t verify_workspace_bytes(int num_seqs, int num_drafts, int64_t) {
-  return (size_t)num_seqs * (num_drafts + 1) * sizeof(RowStat);
+size_t verify_workspace_bytes(int num_seqs, int num_drafts, int64_t vocab) {
+  return verify_layout(num_seqs, num_drafts, vocab).total;
 }
 
 int launch_verify(const VerifyArgs &a, cudaStream_t s) {
