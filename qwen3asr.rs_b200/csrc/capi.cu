@@ -547,6 +547,7 @@ int check_mrope(vasr::MropeAngles *r, const float *cos_table, const float *sin_t
     half += sections[a];
   }
   if (half <= 0 || 2 * half > head_dim) return VASR_PA_EINVAL_SHAPE;
+  if (half > vasr::kMropeMaxHalf) return VASR_PA_ENOT_SUPPORTED;
   if (interleaved)  // axis a's frequencies are a, a + num_axes, ...: all of them must exist
     for (int a = 1; a < num_axes; ++a)
       if (sections[a] > 0 && a + (int64_t)(sections[a] - 1) * num_axes >= half) return VASR_PA_EINVAL_SHAPE;
@@ -559,8 +560,15 @@ int check_mrope(vasr::MropeAngles *r, const float *cos_table, const float *sin_t
   r->max_position = max_position;
   r->half = (int)half;
   r->num_axes = num_axes;
-  r->interleaved = interleaved != 0;
-  for (int a = 0; a < vasr::kMropeMaxAxes; ++a) r->sections[a] = a < num_axes ? sections[a] : 0;
+  int a = 0, end = sections[0];
+  for (int i = 0; i < (int)half; ++i) {
+    if (interleaved) {
+      a = i / num_axes < sections[i % num_axes] ? i % num_axes : 0;
+    } else {
+      while (i >= end) end += sections[++a];
+    }
+    r->axis_bits[i / 16] |= (uint32_t)a << (2 * (i % 16));
+  }
   return VASR_PA_OK;
 }
 
@@ -585,7 +593,7 @@ int32_t vasr_pa_mrope(void *out, int64_t out_token_stride, int64_t out_head_stri
   vasr::MropeArgs a{};
   const int r = check_mrope(&a.rope, cos_table, sin_table, max_position, positions, position_axis_stride,
                             sections, num_axes, interleaved, head_dim);
-  if (r == VASR_PA_EINVAL_SHAPE) return r;
+  if (r == VASR_PA_EINVAL_SHAPE || r == VASR_PA_ENOT_SUPPORTED) return r;
   if (num_tokens == 0) return VASR_PA_OK;
   if (r != VASR_PA_OK) return r;
   // rows of out must not overlap: [tokens, heads, dims] or [heads, tokens, dims] order
@@ -628,7 +636,7 @@ int32_t vasr_pa_fused_qk_norm_mrope_append(
   vasr::MropeAppendArgs a{};
   const int r = check_mrope(&a.rope, cos_table, sin_table, max_position, positions, position_axis_stride,
                             sections, num_axes, interleaved, head_dim);
-  if (r == VASR_PA_EINVAL_SHAPE) return r;
+  if (r == VASR_PA_EINVAL_SHAPE || r == VASR_PA_ENOT_SUPPORTED) return r;
   if (num_tokens == 0) return VASR_PA_OK;
   if (r != VASR_PA_OK) return r;
   if (qkv_token_stride < ((int64_t)num_heads + 2 * (int64_t)num_kv_heads) * head_dim) return VASR_PA_EINVAL_SHAPE;

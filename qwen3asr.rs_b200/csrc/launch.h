@@ -129,9 +129,9 @@ struct FusedRopeArgs {
 };
 int launch_fused_rope(const FusedRopeArgs &a, cudaStream_t s);
 
-// Rotary angles of several position axes (mrope.cu). sections[a] of the half
-// frequencies belong to axis a, one section after another or interleaved.
+// Rotary angles of several position axes (mrope.cu).
 constexpr int kMropeMaxAxes = 4;
+constexpr int kMropeMaxHalf = 256;
 struct MropeAngles {
   const float *cos_table;  // [max_position, half]
   const float *sin_table;
@@ -140,8 +140,7 @@ struct MropeAngles {
   int64_t max_position;
   int half;
   int num_axes;
-  int interleaved;
-  int sections[kMropeMaxAxes];
+  uint32_t axis_bits[kMropeMaxHalf / 16];  // axis of frequency i: 2 bits at 2 (i % 16) of word i / 16
 };
 
 struct MropeAppendArgs {
@@ -270,8 +269,7 @@ struct VerifyArgs {
   int64_t vocab;
   void *workspace;
   // filled by launch_verify
-  int num_chunks;
-  int chunk_elems;
+  int row_chunks;
   void *stats;
   void *bests;
   uint32_t *counters;

@@ -10,6 +10,8 @@
 // The inverse turns by the negative angle; as the rotation is orthogonal it is
 // also the gradient of the forward form. All arithmetic is f32 and each output
 // is rounded once, when it is stored.
+#include <type_traits>
+
 #include "common.cuh"
 #include "launch.h"
 
@@ -20,24 +22,21 @@ constexpr int kWarps = 8;
 constexpr int kMaxDim = 512;
 
 __device__ __forceinline__ int axis_of(const MropeAngles &r, int i) {
-  if (r.interleaved) {
-    const int a = i % r.num_axes;
-    return i / r.num_axes < r.sections[a] ? a : 0;
-  }
-  int a = 0, end = r.sections[0];
-  while (a + 1 < r.num_axes && i >= end) end += r.sections[++a];
-  return a;
+  return (int)(r.axis_bits[i / 16] >> (2 * (i % 16))) & 3;
 }
 
-// cos and sin of frequency i for token t; a position outside the table is
-// clamped to it and recorded.
+// Position of token t on axis a; one outside the table is clamped to it and
+// recorded.
+__device__ __forceinline__ int64_t position_of(const MropeAngles &r, int64_t t, int a) {
+  const int64_t pos = r.positions[a * r.axis_stride + t];
+  if (pos >= 0 && pos < r.max_position) return pos;
+  raise_device_error(VASR_PA_DERR_POSITION_RANGE);
+  return pos < 0 ? 0 : r.max_position - 1;
+}
+
+// cos and sin of frequency i for token t.
 __device__ __forceinline__ float2 angle_of(const MropeAngles &r, int64_t t, int i) {
-  int64_t pos = r.positions[axis_of(r, i) * r.axis_stride + t];
-  if (pos < 0 || pos >= r.max_position) {
-    raise_device_error(VASR_PA_DERR_POSITION_RANGE);
-    pos = pos < 0 ? 0 : r.max_position - 1;
-  }
-  const int64_t at = pos * r.half + i;
+  const int64_t at = position_of(r, t, axis_of(r, i)) * r.half + i;
   return make_float2(__ldg(r.cos_table + at), __ldg(r.sin_table + at));
 }
 
@@ -136,8 +135,249 @@ __global__ void __launch_bounds__(32 * kWarps) mrope_rows_kernel(const MropeArgs
   for (int d = 2 * half + lane; d < p.head_dim; d += 32) y[d] = x[d];
 }
 
+// ------------------------------------------------------------ vector kernels
+// Rows whose D / 2 rotated pairs fall into whole 16-byte chunks: a thread owns
+// chunk c and its partner c + C / 2 of a token's row (C chunks a row), so both
+// halves of its pairs are its own and the norm is a sum over the C / 2 lanes
+// of the row. It loads its cos and sin once and runs over the heads with them.
+template <int kX>
+struct Angles {
+  float c[kX], s[kX];
+  // frequencies [i0, i0 + kX), i0 a multiple of kX (4 or 8): one word of axis bits
+  __device__ __forceinline__ void load(const MropeAngles &r, int64_t t, int i0) {
+    int64_t row[kMropeMaxAxes];
+#pragma unroll
+    for (int a = 0; a < kMropeMaxAxes; ++a) row[a] = a < r.num_axes ? position_of(r, t, a) * r.half + i0 : 0;
+    const uint32_t bits = r.axis_bits[i0 / 16] >> (2 * (i0 % 16));
+#pragma unroll
+    for (int e = 0; e < kX; ++e) {
+      const uint32_t a = bits >> (2 * e) & 3u;
+      const int64_t at = (a == 0 ? row[0] : a == 1 ? row[1] : a == 2 ? row[2] : row[3]) + e;
+      c[e] = __ldg(r.cos_table + at);
+      s[e] = __ldg(r.sin_table + at);
+    }
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ uint4 pack_chunk(const float (&f)[Elem<T>::kX]) {
+  uint4 u;
+  T *e = reinterpret_cast<T *>(&u);
+#pragma unroll
+  for (int i = 0; i < Elem<T>::kX; ++i) e[i] = Elem<T>::from_f32(f[i]);
+  return u;
+}
+
+// kX consecutive dims of one token into a K page (dims d0 .. of a chunk).
+template <typename TC, int kX>
+__device__ __forceinline__ void store_key(TC *at, const float (&f)[kX], float scale) {
+  if constexpr (sizeof(TC) == 1) {
+    uint32_t w[kX / 4];
+#pragma unroll
+    for (int i = 0; i < kX; ++i)
+      reinterpret_cast<__nv_fp8_e4m3 *>(w)[i] = __nv_fp8_e4m3(f[i] / scale);
+    if constexpr (kX == 8) *reinterpret_cast<uint2 *>(at) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint32_t *>(at) = w[0];
+  } else {
+    (void)scale;
+    *reinterpret_cast<uint4 *>(at) = pack_chunk<TC>(f);
+  }
+}
+
+// Tokens of a CTA's tile: 16 in a prompt (or what 8 warps can hold), one
+// warp's worth in a decode step.
+constexpr int tile_tokens(int tokens_per_warp, bool prompt) {
+  return !prompt ? tokens_per_warp : 8 * tokens_per_warp < 16 ? 8 * tokens_per_warp : 16;
+}
+
+// grid = (token tile, part of the heads). Warps split a tile's tokens and its
+// heads. V goes out element by element with the tile's tokens across the
+// lanes: consecutive slots fill a page row's 32-byte sectors whole in one
+// store, and any other slots need no case of their own.
+template <typename T, typename TC, int D, bool kPrompt>
+__global__ void __launch_bounds__(32 * kWarps) mrope_append_tile_kernel(const MropeAppendArgs p) {
+  pdl_launch_dependents();  // a decode behind this kernel reads nothing it writes before it has ended
+  constexpr int kX = Elem<T>::kX, C = D / kX, L = C / 2, kPerWarp = 32 / L;
+  constexpr int kTile = tile_tokens(kPerWarp, kPrompt), kGroups = kTile / kPerWarp, kHeadLanes = kWarps / kGroups;
+  constexpr int kXc = Elem<TC>::kX;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int shift = 31 - __clz(p.block_size);
+  const int64_t tile0 = (int64_t)blockIdx.x * kTile;
+  const int parts = gridDim.y, part = blockIdx.y;
+  auto slot_of = [&](int64_t t) -> int64_t {
+    if (t >= p.num_tokens) return -1;
+    const int64_t slot = p.slot_mapping[t];
+    if (slot < p.num_blocks << shift) return slot;
+    raise_device_error(VASR_PA_DERR_SLOT_RANGE);
+    return -1;
+  };
+  {  // ---- q and k
+    const int c = lane % L;
+    const int64_t t = tile0 + (warp % kGroups) * kPerWarp + lane / L;
+    const bool live = t < p.num_tokens;
+    const int64_t tt = live ? t : p.num_tokens - 1;  // lanes past the end follow, for the shuffles
+    const T *src = static_cast<const T *>(p.qkv) + tt * p.qkv_token_stride + c * kX;
+    const int64_t slot = slot_of(t);
+    Angles<kX> ang;
+    ang.load(p.rope, tt, c * kX);
+    const float k_scale = p.k_scale ? __ldg(p.k_scale) : 1.f;
+    auto head_range = [&](int first, int count, const T *weight, bool is_q) {
+      uint4 w0 = make_uint4(0, 0, 0, 0), w1 = w0;
+      if (weight) {
+        w0 = __ldg(reinterpret_cast<const uint4 *>(weight + c * kX));
+        w1 = __ldg(reinterpret_cast<const uint4 *>(weight + c * kX + D / 2));
+      }
+#pragma unroll 2
+      for (int h = warp / kGroups + kHeadLanes * part; h < count; h += kHeadLanes * parts) {
+        const T *row = src + (int64_t)(first + h) * D;
+        float a[kX], b[kX];
+        unpack_chunk<T>(__ldg(reinterpret_cast<const uint4 *>(row)), a);
+        unpack_chunk<T>(__ldg(reinterpret_cast<const uint4 *>(row + D / 2)), b);
+        if (weight) {
+          float ss = 0.f, wa[kX], wb[kX];
+#pragma unroll
+          for (int e = 0; e < kX; ++e) ss = fmaf(a[e], a[e], fmaf(b[e], b[e], ss));
+          const float inv = rsqrtf(warp_sum_xor(ss, L) / (float)D + p.eps);
+          unpack_chunk<T>(w0, wa);
+          unpack_chunk<T>(w1, wb);
+#pragma unroll
+          for (int e = 0; e < kX; ++e) {
+            a[e] *= inv * wa[e];
+            b[e] *= inv * wb[e];
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < kX; ++e) {
+          const float x = a[e];
+          a[e] = x * ang.c[e] - b[e] * ang.s[e];
+          b[e] = b[e] * ang.c[e] + x * ang.s[e];
+        }
+        if (is_q) {
+          if (live) {
+            T *q = static_cast<T *>(p.q_out) + (t * p.num_heads + h) * D + c * kX;
+            *reinterpret_cast<uint4 *>(q) = pack_chunk<T>(a);
+            *reinterpret_cast<uint4 *>(q + D / 2) = pack_chunk<T>(b);
+          }
+        } else if (slot >= 0) {
+          const int64_t page = (slot >> shift) * p.num_kv_heads + h;
+          const int off = (int)(slot & (p.block_size - 1));
+          auto place = [&](int d) {
+            return static_cast<TC *>(p.key_cache) + (((page * (D / kXc) + d / kXc) << shift) + off) * kXc + d % kXc;
+          };
+          store_key<TC, kX>(place(c * kX), a, k_scale);
+          store_key<TC, kX>(place(c * kX + D / 2), b, k_scale);
+          if (p.score_cache && c == 0) p.score_cache[(page << shift) + off] = 0.f;
+        }
+      }
+    };
+    head_range(0, p.num_heads, static_cast<const T *>(p.q_norm_weight), true);
+    head_range(p.num_heads, p.num_kv_heads, static_cast<const T *>(p.k_norm_weight), false);
+  }
+  {  // ---- v: item = (head, group of chunks), the tile's tokens across the lanes
+    constexpr int kChunks = 32 / kTile, kItems = C / kChunks;
+    const int64_t t = tile0 + lane % kTile;
+    const int cc = lane / kTile;
+    const int64_t slot = slot_of(t);
+    if (slot < 0) return;
+    const T *src = static_cast<const T *>(p.qkv) + t * p.qkv_token_stride + (int64_t)(p.num_heads + p.num_kv_heads) * D;
+    TC *dst = static_cast<TC *>(p.value_cache) + (((slot >> shift) * p.num_kv_heads * D) << shift) +
+              (slot & (p.block_size - 1));
+    const float v_scale = p.v_scale ? __ldg(p.v_scale) : 1.f;
+#pragma unroll 2
+    for (int i = warp + kWarps * part; i < p.num_kv_heads * kItems; i += kWarps * parts) {
+      const int d = (i * kChunks + cc) * kX;  // dim of the token's V row, over the heads
+      const uint4 raw = __ldg(reinterpret_cast<const uint4 *>(src + d));
+      TC *at = dst + ((int64_t)d << shift);
+      if constexpr (std::is_same<T, TC>::value) {
+        const T *e = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+        for (int k = 0; k < kX; ++k) at[(int64_t)k << shift] = e[k];
+      } else {
+        float f[kX];
+        unpack_chunk<T>(raw, f);
+#pragma unroll
+        for (int k = 0; k < kX; ++k) at[(int64_t)k << shift] = __nv_fp8_e4m3(f[k] / v_scale);
+      }
+    }
+  }
+}
+
+// x [T, H, D] turned: a warp per C / 2-lane token group and part of the heads.
+template <typename T, int D>
+__global__ void __launch_bounds__(32 * kWarps) mrope_tile_kernel(const MropeArgs p) {
+  constexpr int kX = Elem<T>::kX, L = D / kX / 2, kTile = 32 * kWarps / L;  // tokens of a CTA
+  const int c = threadIdx.x % L;
+  const int64_t t = (int64_t)blockIdx.x * kTile + threadIdx.x / L;
+  if (t >= p.num_tokens) return;
+  Angles<kX> ang;
+  ang.load(p.rope, t, c * kX);
+#pragma unroll
+  for (int e = 0; e < kX; ++e)
+    if (p.inverse) ang.s[e] = -ang.s[e];
+  const T *x = static_cast<const T *>(p.x) + t * p.x_token_stride + c * kX;
+  T *y = static_cast<T *>(p.out) + t * p.out_token_stride + c * kX;
+#pragma unroll 4
+  for (int h = blockIdx.y; h < p.num_heads; h += gridDim.y) {
+    float a[kX], b[kX];
+    // plain loads: y may be x
+    unpack_chunk<T>(*reinterpret_cast<const uint4 *>(x + h * p.x_head_stride), a);
+    unpack_chunk<T>(*reinterpret_cast<const uint4 *>(x + h * p.x_head_stride + D / 2), b);
+#pragma unroll
+    for (int e = 0; e < kX; ++e) {
+      const float v = a[e];
+      a[e] = v * ang.c[e] - b[e] * ang.s[e];
+      b[e] = b[e] * ang.c[e] + v * ang.s[e];
+    }
+    *reinterpret_cast<uint4 *>(y + h * p.out_head_stride) = pack_chunk<T>(a);
+    *reinterpret_cast<uint4 *>(y + h * p.out_head_stride + D / 2) = pack_chunk<T>(b);
+  }
+}
+
+bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+constexpr int kPromptTokens = 1024;
+constexpr int kTargetCtas = 4 * 148;
+
+template <typename T, typename TC, int D, bool kPrompt>
+int launch_append_tile(const MropeAppendArgs &a, cudaStream_t s) {
+  constexpr int kPerWarp = 32 / (D / Elem<T>::kX / 2);
+  constexpr int kTile = tile_tokens(kPerWarp, kPrompt), kHeadLanes = kWarps / (kTile / kPerWarp);
+  const int64_t tiles = (a.num_tokens + kTile - 1) / kTile;
+  const int most = (a.num_heads + kHeadLanes - 1) / kHeadLanes;
+  int64_t parts = kTargetCtas / tiles;
+  parts = parts < 1 ? 1 : parts > most ? most : parts;
+  if (tiles > 0x7fffffff || parts > 65535) return VASR_PA_EINVAL_SHAPE;
+  mrope_append_tile_kernel<T, TC, D, kPrompt><<<dim3((unsigned)tiles, (unsigned)parts), 32 * kWarps, 0, s>>>(a);
+  return cudaPeekAtLastError() == cudaSuccess ? VASR_PA_OK : VASR_PA_ELAUNCH;
+}
+
+template <typename T, typename TC, int D>
+int launch_append_d(const MropeAppendArgs &a, cudaStream_t s) {
+  if (a.num_tokens >= kPromptTokens) return launch_append_tile<T, TC, D, true>(a, s);
+  return launch_append_tile<T, TC, D, false>(a, s);
+}
+
+template <typename T, int D>
+int launch_tile(const MropeArgs &a, cudaStream_t s) {
+  constexpr int kTile = 32 * kWarps / (D / Elem<T>::kX / 2);
+  const int64_t tiles = (a.num_tokens + kTile - 1) / kTile;
+  int64_t parts = kTargetCtas / tiles;
+  parts = parts < 1 ? 1 : parts > a.num_heads ? a.num_heads : parts;
+  if (tiles > 0x7fffffff || parts > 65535) return VASR_PA_EINVAL_SHAPE;
+  mrope_tile_kernel<T, D><<<dim3((unsigned)tiles, (unsigned)parts), 32 * kWarps, 0, s>>>(a);
+  return cudaPeekAtLastError() == cudaSuccess ? VASR_PA_OK : VASR_PA_ELAUNCH;
+}
+
 template <typename T, typename TC>
 int launch_append_tc(const MropeAppendArgs &a, cudaStream_t s) {
+  if (2 * a.rope.half == a.head_dim && aligned16(a.qkv) && (a.qkv_token_stride * (int64_t)sizeof(T)) % 16 == 0 &&
+      aligned16(a.q_out) && aligned16(a.q_norm_weight) && aligned16(a.k_norm_weight)) {
+    switch (a.head_dim) {
+      case 64: return launch_append_d<T, TC, 64>(a, s);
+      case 128: return launch_append_d<T, TC, 128>(a, s);
+      case 256: return launch_append_d<T, TC, 256>(a, s);
+      default: break;
+    }
+  }
   const int64_t warps = a.num_tokens * (a.num_heads + 2 * a.num_kv_heads);
   const int64_t ctas = (warps + kWarps - 1) / kWarps;
   if (ctas > 0x7fffffff) return VASR_PA_EINVAL_SHAPE;
@@ -153,6 +393,16 @@ int launch_append_t(const MropeAppendArgs &a, cudaStream_t s) {
 
 template <typename T>
 int launch_rows_t(const MropeArgs &a, cudaStream_t s) {
+  auto whole = [](int64_t stride) { return stride * (int64_t)sizeof(T) % 16 == 0; };
+  if (2 * a.rope.half == a.head_dim && aligned16(a.x) && aligned16(a.out) && whole(a.x_token_stride) &&
+      whole(a.x_head_stride) && whole(a.out_token_stride) && whole(a.out_head_stride)) {
+    switch (a.head_dim) {
+      case 64: return launch_tile<T, 64>(a, s);
+      case 128: return launch_tile<T, 128>(a, s);
+      case 256: return launch_tile<T, 256>(a, s);
+      default: break;
+    }
+  }
   const int64_t ctas = (a.num_tokens * a.num_heads + kWarps - 1) / kWarps;
   if (ctas > 0x7fffffff) return VASR_PA_EINVAL_SHAPE;
   mrope_rows_kernel<T><<<(unsigned)ctas, 32 * kWarps, 0, s>>>(a);

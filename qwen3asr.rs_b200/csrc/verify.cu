@@ -13,20 +13,23 @@
 // n's argmax. Lowest index on equal values; NaN logits count as -inf.
 //
 // Two launches. The first gives every chunk of every row its maximum and its
-// sum of exp((x - max) / T) in one pass: a thread keeps its 32 logits in
+// sum of exp((x - max) / T) in one pass: a thread keeps its logits in
 // registers between the maximum and the sum. The second, a programmatic
 // dependent of the first, has a CTA per chunk of a sequence's vocabulary: it
 // loads its noise and the drafts' logits early, joins the rows' chunks and
 // decides on its own copy (a few hundred bytes), runs the race over its chunk
 // of row n, and the last CTA of the sequence takes the winner. Only the row
 // that is drawn from is read twice, the second time from L2.
+#include <type_traits>
+
 #include "common.cuh"
 #include "launch.h"
 
 namespace vasr {
 namespace {
 
-constexpr int kPerThread = 32;  // logits a thread keeps in registers
+constexpr int kRowElems = 32;   // logits a thread of the first launch keeps in registers
+constexpr int kEmitElems = 16;  // logits, drafter's values and noise each of the second's (80 registers)
 constexpr int kMaxThreads = 256;
 
 // One chunk of a row: its maximum (and, for greedy rows, the first place of
@@ -60,10 +63,23 @@ __device__ __forceinline__ float temperature_of(const VerifyArgs &p, int b) {
 __device__ __forceinline__ int drafts_of(const VerifyArgs &p, int b) {
   return p.draft_lens ? min(max(p.draft_lens[b], 0), p.num_drafts) : p.num_drafts;
 }
-// exp((x - max) / T) with c = log2(e) / T; the entries at an infinite maximum
-// share the mass, and -inf weighs nothing.
+// exp((x - max) / T) with c = log2(e) / T. exp2 in its one-instruction form
+// (2 ulp): the product's own rounding is no smaller, and the precise form's
+// range checks took a third of the kernels' instructions. weight_of also
+// holds where max is +inf (the entries there share the mass) or 1 / T is.
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float plain_weight(float x, float max, float c) { return exp2_approx((x - max) * c); }
 __device__ __forceinline__ float weight_of(float x, float max, float c) {
-  return x == max ? 1.f : exp2f((x - max) * c);
+  return x == max ? 1.f : x == x ? plain_weight(x, max, c) : 0.f;
 }
 
 // A thread's elements of a chunk of a row: groups of 8, group tid + k threads
@@ -71,8 +87,7 @@ __device__ __forceinline__ float weight_of(float x, float max, float c) {
 // Vector loads where the group is 16-byte aligned and whole, else one by one
 // (what lies past the chunk reads as 0).
 constexpr int kGroup = 8;
-constexpr int kGroups = kPerThread / kGroup;
-template <typename T>
+template <typename T, int kGroups>
 struct Held {
   static constexpr int kVec = 16 / (int)sizeof(T);
   static constexpr int kVecs = kGroup / kVec;
@@ -108,38 +123,58 @@ struct Held {
       for (int i = 0; i < kVec; ++i) out[v * kVec + i] = f[i];
     }
   }
+  // the largest element of group k; NaN is passed over
+  __device__ __forceinline__ float group_max(int k) const {
+    if constexpr (sizeof(T) == 2) {
+      using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+      const T2 *h = reinterpret_cast<const T2 *>(&raw[k][0]);
+      const T2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+      return fmaxf(Elem<T>::to_f32(m.x), Elem<T>::to_f32(m.y));
+    } else {
+      float v[kGroup];
+      group(k, v);
+      float m = v[0];
+#pragma unroll
+      for (int i = 1; i < kGroup; ++i) m = fmaxf(m, v[i]);
+      return m;
+    }
+  }
 };
+
+// The guarded forms for a chunk's rest (fewer than 8 elements of a group) and
+// for logits that are not finite.
+template <typename T, int kGroups, typename F>
+__device__ __forceinline__ void each_guarded(const Held<T, kGroups> &x, int len, int tid, int threads, F f) {
+  for (int k = 0; k < kGroups; ++k) {
+    float v[kGroup];
+    x.group(k, v);
+    const int j = (tid + k * threads) * kGroup;
+#pragma unroll
+    for (int i = 0; i < kGroup; ++i)
+      if (j + i < len && v[i] == v[i]) f(v[i], j + i);
+  }
+}
 
 template <typename T>
 __global__ void __launch_bounds__(kMaxThreads) verify_rows_kernel(const VerifyArgs p) {
   pdl_launch_dependents();
+  constexpr int kGroups = kRowElems / kGroup;
   const int chunk = blockIdx.x, i = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, threads = blockDim.x;
   if (i > drafts_of(p, b)) return;
-  const int64_t lo = (int64_t)chunk * p.chunk_elems;
-  const int len = (int)min((int64_t)p.chunk_elems, p.vocab - lo);
+  const int size = threads * kRowElems;
+  const int64_t lo = (int64_t)chunk * size;
+  const int len = (int)min((int64_t)size, p.vocab - lo);
   const T *row = static_cast<const T *>(p.logits) + b * p.logits_seq_stride + i * p.logits_row_stride + lo;
-  Held<T> x;
+  Held<T, kGroups> x;
   x.load(row, len, tid, threads);
   const float t = temperature_of(p, b);
-  // f(logit, index) for the thread's elements; NaN counts as -inf
-  auto each = [&](auto f) {
-#pragma unroll
-    for (int k = 0; k < kGroups; ++k) {
-      const int j = (tid + k * threads) * kGroup;
-      float v[kGroup];
-      x.group(k, v);
-      if (j + kGroup <= len) {
-#pragma unroll
-        for (int i = 0; i < kGroup; ++i) f(fmaxf(v[i], -INFINITY), j + i);
-      } else {
-#pragma unroll
-        for (int i = 0; i < kGroup; ++i)
-          if (j + i < len) f(fmaxf(v[i], -INFINITY), j + i);
-      }
-    }
-  };
   float m = -INFINITY;
-  each([&](float v, int) { m = fmaxf(m, v); });
+  if (len == size) {
+#pragma unroll
+    for (int k = 0; k < kGroups; ++k) m = fmaxf(m, x.group_max(k));
+  } else {
+    each_guarded(x, len, tid, threads, [&](float v, int) { m = fmaxf(m, v); });
+  }
   __shared__ float part[kMaxThreads / 32];
   __shared__ uint32_t s_arg;
   const int warps = threads >> 5;
@@ -152,7 +187,21 @@ __global__ void __launch_bounds__(kMaxThreads) verify_rows_kernel(const VerifyAr
   float sum = 0.f;
   if (t > 0.f) {
     const float c = kLog2e / t;
-    if (m > -INFINITY) each([&](float v, int) { sum += weight_of(v, m, c); });
+    if (m > -INFINITY) {
+      if (len == size) {
+#pragma unroll
+        for (int k = 0; k < kGroups; ++k) {
+          float v[kGroup];
+          x.group(k, v);
+#pragma unroll
+          for (int e = 0; e < kGroup; ++e) sum += plain_weight(v[e], m, c);
+        }
+      }
+      if (len != size || !(sum == sum)) {
+        sum = 0.f;
+        each_guarded(x, len, tid, threads, [&](float v, int) { sum += weight_of(v, m, c); });
+      }
+    }
     sum = warp_sum_xor(sum, 32);
     if ((tid & 31) == 0) part[tid >> 5] = sum;
     __syncthreads();
@@ -160,7 +209,7 @@ __global__ void __launch_bounds__(kMaxThreads) verify_rows_kernel(const VerifyAr
     for (int w = 0; w < warps; ++w) sum += part[w];
   } else {
     uint32_t first = kNone;
-    each([&](float v, int j) {
+    each_guarded(x, len, tid, threads, [&](float v, int j) {
       if (v == m) first = min(first, (uint32_t)j);
     });
     if (first != kNone) atomicMin(&s_arg, first);
@@ -168,7 +217,7 @@ __global__ void __launch_bounds__(kMaxThreads) verify_rows_kernel(const VerifyAr
   }
   if (tid == 0) {
     ChunkStat *out = static_cast<ChunkStat *>(p.stats);
-    out[((int64_t)b * (p.num_drafts + 1) + i) * p.num_chunks + chunk] =
+    out[((int64_t)b * (p.num_drafts + 1) + i) * p.row_chunks + chunk] =
         ChunkStat{m, sum, s_arg != kNone ? (uint32_t)lo + s_arg : 0u, 0u};
   }
 }
@@ -176,15 +225,15 @@ __global__ void __launch_bounds__(kMaxThreads) verify_rows_kernel(const VerifyAr
 // A whole row from its chunks, by one warp.
 __device__ __forceinline__ ChunkStat join_chunks(const VerifyArgs &p, int64_t row, float t) {
   const int lane = threadIdx.x & 31;
-  const ChunkStat *s = static_cast<const ChunkStat *>(p.stats) + row * p.num_chunks;
+  const ChunkStat *s = static_cast<const ChunkStat *>(p.stats) + row * p.row_chunks;
   Best top{-INFINITY, kNone};
-  for (int c = lane; c < p.num_chunks; c += 32)
+  for (int c = lane; c < p.row_chunks; c += 32)
     if (s[c].max > -INFINITY) top = better(top, Best{s[c].max, s[c].arg});
   top = warp_best(top);
   float sum = 0.f;
   if (t > 0.f && top.v > -INFINITY) {
     const float k = kLog2e / t;
-    for (int c = lane; c < p.num_chunks; c += 32)
+    for (int c = lane; c < p.row_chunks; c += 32)
       if (s[c].sum != 0.f) sum = fmaf(s[c].sum, weight_of(s[c].max, top.v, k), sum);
     sum = warp_sum_xor(sum, 32);
   }
@@ -192,7 +241,7 @@ __device__ __forceinline__ ChunkStat join_chunks(const VerifyArgs &p, int64_t ro
 }
 
 template <typename T, typename TQ>
-__global__ void __launch_bounds__(kMaxThreads) verify_emit_kernel(const VerifyArgs p) {
+__global__ void __launch_bounds__(kMaxThreads, 4) verify_emit_kernel(const VerifyArgs p) {
   extern __shared__ ChunkStat s_row[];  // [num_drafts + 1]
   __shared__ int s_fail;
   __shared__ Best part[kMaxThreads / 32];
@@ -204,11 +253,13 @@ __global__ void __launch_bounds__(kMaxThreads) verify_emit_kernel(const VerifyAr
   const T *rows = static_cast<const T *>(p.logits) + b * p.logits_seq_stride;
   const TQ *probs = p.draft_probs ? static_cast<const TQ *>(p.draft_probs) + b * p.probs_seq_stride : nullptr;
   const int32_t *drafts = p.draft_tokens + (int64_t)b * p.num_drafts;
-  const int64_t lo = (int64_t)chunk * p.chunk_elems;
-  const int len = (int)min((int64_t)p.chunk_elems, p.vocab - lo);
+  constexpr int kGroups = kEmitElems / kGroup;
+  const int size = threads * kEmitElems;
+  const int64_t lo = (int64_t)chunk * size;
+  const int len = (int)min((int64_t)size, p.vocab - lo);
   if (tid == 0) s_fail = k;
   // inputs that the first launch does not write
-  Held<float> race;
+  Held<float, kGroups> race;
   if (t > 0.f) race.load(p.race + b * p.race_seq_stride + lo, len, tid, threads);
   int32_t x0 = -1;
   float logit0 = -INFINITY, q0 = 1.f, u0 = 0.f;
@@ -254,48 +305,54 @@ __global__ void __launch_bounds__(kMaxThreads) verify_emit_kernel(const VerifyAr
   const bool drawn = t > 0.f && s.max > -INFINITY;
   uint32_t next = s.arg;
   if (drawn) {
-    // ---- the race over this chunk; a quotient is taken only where it wins
-    Held<T> x;
+    // ---- the race over this chunk. The quotient takes one reciprocal
+    // instruction (1 ulp); only r / e > 0 can win, so NaN and r <= 0 drop out.
+    Held<T, kGroups> x;
     x.load(row + lo, len, tid, threads);
-    Held<TQ> q;
+    Held<TQ, kGroups> q;
     if (qrow) q.load(qrow + lo, len, tid, threads);
     const float inv = 1.f / s.sum;
-    Best best{-1.f, kNone};
+    const bool finite = s.max < INFINITY && c < INFINITY;
+    const int skip = failed >= lo && failed < lo + len && !qrow ? (int)(failed - lo) : -1;
+    Best best{0.f, kNone};
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
       const int j = (tid + g * threads) * kGroup;
       float w[kGroup], e[kGroup], qv[kGroup];
       x.group(g, w);
       race.group(g, e);
-      if (qrow) q.group(g, qv);
+      if (qrow) {
+        q.group(g, qv);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i) qv[i] = 0.f;
+      }
 #pragma unroll
       for (int i = 0; i < kGroup; ++i) {
-        float r = weight_of(fmaxf(w[i], -INFINITY), s.max, c) * inv;
-        if (qrow) r -= qv[i];
-        else if (lo + j + i == failed) r = 0.f;
-        if (j + i < len && r > 0.f && r > best.v * e[i]) {
-          const float a = r / e[i];
-          if (a > best.v) best = Best{a, (uint32_t)(lo + j + i)};
-        }
+        const float pw = finite ? plain_weight(w[i], s.max, c) : weight_of(w[i], s.max, c);
+        float a = fmaf(pw, inv, -qv[i]) * rcp_approx(e[i]);
+        if (j + i >= len || j + i == skip) a = 0.f;
+        if (a > best.v) best = Best{a, (uint32_t)(j + i)};
       }
     }
+    if (best.i != kNone) best.i += (uint32_t)lo;
     best = warp_best(best);
     if (lane == 0) part[warp] = best;
     __syncthreads();
     if (tid == 0) {
       for (int w = 1; w < warps; ++w) best = better(best, part[w]);
-      Best *slots = static_cast<Best *>(p.bests) + (int64_t)b * p.num_chunks;
+      Best *slots = static_cast<Best *>(p.bests) + (int64_t)b * gridDim.x;
       slots[chunk] = best;
       __threadfence();
-      s_last = atomicAdd(p.counters + b, 1u) == (uint32_t)p.num_chunks - 1;
+      s_last = atomicAdd(p.counters + b, 1u) == gridDim.x - 1;
       __threadfence();
     }
     __syncthreads();
     if (!s_last) return;
     // ---- the sequence's last CTA: the winner over all chunks
-    best = Best{-1.f, kNone};
-    const Best *slots = static_cast<const Best *>(p.bests) + (int64_t)b * p.num_chunks;
-    for (int i = tid; i < p.num_chunks; i += threads) best = better(best, Best{__ldcg(&slots[i].v), __ldcg(&slots[i].i)});
+    best = Best{0.f, kNone};
+    const Best *slots = static_cast<const Best *>(p.bests) + (int64_t)b * gridDim.x;
+    for (int i = tid; i < (int)gridDim.x; i += threads) best = better(best, Best{__ldcg(&slots[i].v), __ldcg(&slots[i].i)});
     best = warp_best(best);
     if (lane == 0) part[warp] = best;
     __syncthreads();
@@ -305,9 +362,8 @@ __global__ void __launch_bounds__(kMaxThreads) verify_emit_kernel(const VerifyAr
       __syncthreads();
       const float *noise = p.race + b * p.race_seq_stride;
       for (int64_t v = tid; v < p.vocab; v += threads) {
-        const float pv = weight_of(fmaxf(Elem<T>::to_f32(row[v]), -INFINITY), s.max, c) * inv;
-        const float a = pv / noise[v];
-        if (pv > 0.f && a > best.v) best = Best{a, (uint32_t)v};
+        const float a = weight_of(Elem<T>::to_f32(row[v]), s.max, c) * inv * rcp_approx(noise[v]);
+        if (a > best.v) best = Best{a, (uint32_t)v};
       }
       best = warp_best(best);
       if (lane == 0) part[warp] = best;
@@ -333,18 +389,19 @@ int chunk_threads(int num_seqs, int num_drafts, int64_t vocab) {
 }
 
 struct VerifyLayout {
-  int threads, num_chunks;
+  int threads, row_chunks, emit_chunks;
   size_t off_stats, off_bests, total;
 };
 constexpr size_t kCounterBytes = 65536 * sizeof(uint32_t);  // one per sequence, left at zero
 VerifyLayout verify_layout(int num_seqs, int num_drafts, int64_t vocab) {
   VerifyLayout l;
   l.threads = chunk_threads(num_seqs, num_drafts, vocab);
-  const int64_t per = (int64_t)l.threads * kPerThread;
-  l.num_chunks = (int)((vocab + per - 1) / per);
+  auto chunks = [&](int elems) { return (int)((vocab + l.threads * elems - 1) / (l.threads * elems)); };
+  l.row_chunks = chunks(kRowElems);
+  l.emit_chunks = chunks(kEmitElems);
   l.off_stats = kCounterBytes;
-  l.off_bests = l.off_stats + (size_t)num_seqs * (num_drafts + 1) * l.num_chunks * sizeof(ChunkStat);
-  l.total = l.off_bests + (size_t)num_seqs * l.num_chunks * sizeof(Best);
+  l.off_bests = l.off_stats + (size_t)num_seqs * (num_drafts + 1) * l.row_chunks * sizeof(ChunkStat);
+  l.total = l.off_bests + (size_t)num_seqs * l.emit_chunks * sizeof(Best);
   return l;
 }
 
@@ -355,12 +412,11 @@ int launch_verify_tq(VerifyArgs a, cudaStream_t s) {
   a.counters = reinterpret_cast<uint32_t *>(ws);
   a.stats = ws + l.off_stats;
   a.bests = ws + l.off_bests;
-  a.num_chunks = l.num_chunks;
-  a.chunk_elems = l.threads * kPerThread;
-  verify_rows_kernel<T><<<dim3((unsigned)l.num_chunks, (unsigned)a.num_drafts + 1, (unsigned)a.num_seqs),
+  a.row_chunks = l.row_chunks;
+  verify_rows_kernel<T><<<dim3((unsigned)l.row_chunks, (unsigned)a.num_drafts + 1, (unsigned)a.num_seqs),
                           (unsigned)l.threads, 0, s>>>(a);
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)l.num_chunks, (unsigned)a.num_seqs);
+  cfg.gridDim = dim3((unsigned)l.emit_chunks, (unsigned)a.num_seqs);
   cfg.blockDim = dim3((unsigned)l.threads);
   cfg.dynamicSmemBytes = (size_t)(a.num_drafts + 1) * sizeof(ChunkStat);
   cfg.stream = s;
