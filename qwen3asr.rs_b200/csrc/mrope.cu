@@ -34,6 +34,14 @@ __device__ __forceinline__ int64_t position_of(const MropeAngles &r, int64_t t, 
   return pos < 0 ? 0 : r.max_position - 1;
 }
 
+// d = a b for two f32 pairs, one packed instruction
+__device__ __forceinline__ void mul2(float &d0, float &d1, float a0, float a1, float b0, float b1) {
+  asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+      "mul.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+
 // cos and sin of frequency i for token t.
 __device__ __forceinline__ float2 angle_of(const MropeAngles &r, int64_t t, int i) {
   const int64_t at = position_of(r, t, axis_of(r, i)) * r.half + i;
@@ -143,18 +151,37 @@ __global__ void __launch_bounds__(32 * kWarps) mrope_rows_kernel(const MropeArgs
 template <int kX>
 struct Angles {
   float c[kX], s[kX];
-  // frequencies [i0, i0 + kX), i0 a multiple of kX (4 or 8): one word of axis bits
+  // frequencies [i0, i0 + kX), i0 a multiple of kX (4 or 8): one word of axis
+  // bits; every axis' row in vectors (16-byte aligned), then a choice per frequency
   __device__ __forceinline__ void load(const MropeAngles &r, int64_t t, int i0) {
-    int64_t row[kMropeMaxAxes];
-#pragma unroll
-    for (int a = 0; a < kMropeMaxAxes; ++a) row[a] = a < r.num_axes ? position_of(r, t, a) * r.half + i0 : 0;
     const uint32_t bits = r.axis_bits[i0 / 16] >> (2 * (i0 % 16));
 #pragma unroll
-    for (int e = 0; e < kX; ++e) {
-      const uint32_t a = bits >> (2 * e) & 3u;
-      const int64_t at = (a == 0 ? row[0] : a == 1 ? row[1] : a == 2 ? row[2] : row[3]) + e;
-      c[e] = __ldg(r.cos_table + at);
-      s[e] = __ldg(r.sin_table + at);
+    for (int a = 0; a < kMropeMaxAxes; ++a) {
+      if (a >= r.num_axes) break;
+      const int64_t at = position_of(r, t, a) * r.half + i0;
+#pragma unroll
+      for (int v = 0; v < kX / 4; ++v) {
+        const float4 cv = __ldg(reinterpret_cast<const float4 *>(r.cos_table + at) + v);
+        const float4 sv = __ldg(reinterpret_cast<const float4 *>(r.sin_table + at) + v);
+        const float cf[4] = {cv.x, cv.y, cv.z, cv.w}, sf[4] = {sv.x, sv.y, sv.z, sv.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool mine = a == 0 || (bits >> (2 * (4 * v + e)) & 3u) == (uint32_t)a;
+          c[4 * v + e] = mine ? cf[e] : c[4 * v + e];
+          s[4 * v + e] = mine ? sf[e] : s[4 * v + e];
+        }
+      }
+    }
+  }
+  // (a, b) turned, all pairs; sums and products of two frequencies at a time
+  __device__ __forceinline__ void turn(float (&a)[kX], float (&b)[kX]) const {
+#pragma unroll
+    for (int e = 0; e < kX; e += 2) {
+      float x0 = a[e], x1 = a[e + 1], y0 = b[e], y1 = b[e + 1];
+      mul2(a[e], a[e + 1], x0, x1, c[e], c[e + 1]);
+      mul2(b[e], b[e + 1], y0, y1, c[e], c[e + 1]);
+      fma2(a[e], a[e + 1], y0, y1, -s[e], -s[e + 1]);
+      fma2(b[e], b[e + 1], x0, x1, s[e], s[e + 1]);
     }
   }
 };
@@ -162,9 +189,17 @@ struct Angles {
 template <typename T>
 __device__ __forceinline__ uint4 pack_chunk(const float (&f)[Elem<T>::kX]) {
   uint4 u;
-  T *e = reinterpret_cast<T *>(&u);
+  if constexpr (sizeof(T) == 4) {
+    u = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  } else {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    T2 *e = reinterpret_cast<T2 *>(&u);
 #pragma unroll
-  for (int i = 0; i < Elem<T>::kX; ++i) e[i] = Elem<T>::from_f32(f[i]);
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same<T, __half>::value) e[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+      else e[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+    }
+  }
   return u;
 }
 
@@ -184,26 +219,42 @@ __device__ __forceinline__ void store_key(TC *at, const float (&f)[kX], float sc
   }
 }
 
-// Tokens of a CTA's tile: 16 in a prompt (or what 8 warps can hold), one
-// warp's worth in a decode step.
+// A prompt's CTA has a tile of 16 tokens and a warp for each warp's worth of
+// them (at most 8), which runs over all heads of its part with one set of
+// angles; a decode step's CTA one warp's worth of tokens and 8 warps that
+// split the heads.
 constexpr int tile_tokens(int tokens_per_warp, bool prompt) {
   return !prompt ? tokens_per_warp : 8 * tokens_per_warp < 16 ? 8 * tokens_per_warp : 16;
 }
+template <typename T, int D>
+constexpr int tile_warps(bool prompt) {
+  return prompt ? tile_tokens(64 / (D / Elem<T>::kX), true) / (64 / (D / Elem<T>::kX)) : 8;
+}
 
-// grid = (token tile, part of the heads). Warps split a tile's tokens and its
-// heads. V goes out element by element with the tile's tokens across the
+// Prompts: the part's heads of the tile's rows arrive by one bulk copy a token
+// (a token's heads are adjacent), so that the bytes in flight cost shared
+// memory and not registers; rows are 16 bytes apart modulo 128 to spread banks.
+constexpr int kPartBytes = 2048;  // of one token's row
+template <typename T, int D>
+constexpr int part_heads() { return kPartBytes / (D * (int)sizeof(T)) > 0 ? kPartBytes / (D * (int)sizeof(T)) : 1; }
+template <typename T, int D>
+constexpr int part_pitch() { return part_heads<T, D>() * D * (int)sizeof(T) + 16; }
+
+// grid = (token tile, part): the first qk_parts parts share the tile's q and k
+// heads, the others its V. Warps split a tile's tokens and its heads. V goes out element by element with the tile's tokens across the
 // lanes: consecutive slots fill a page row's 32-byte sectors whole in one
 // store, and any other slots need no case of their own.
 template <typename T, typename TC, int D, bool kPrompt>
-__global__ void __launch_bounds__(32 * kWarps) mrope_append_tile_kernel(const MropeAppendArgs p) {
+__global__ void __launch_bounds__(32 * tile_warps<T, D>(kPrompt)) mrope_append_tile_kernel(const MropeAppendArgs p,
+                                                                                          int qk_parts) {
   pdl_launch_dependents();  // a decode behind this kernel reads nothing it writes before it has ended
   constexpr int kX = Elem<T>::kX, C = D / kX, L = C / 2, kPerWarp = 32 / L;
-  constexpr int kTile = tile_tokens(kPerWarp, kPrompt), kGroups = kTile / kPerWarp, kHeadLanes = kWarps / kGroups;
+  constexpr int kTile = tile_tokens(kPerWarp, kPrompt), kGroups = kTile / kPerWarp;
+  constexpr int kCtaWarps = tile_warps<T, D>(kPrompt), kHeadLanes = kCtaWarps / kGroups;
   constexpr int kXc = Elem<TC>::kX;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int shift = 31 - __clz(p.block_size);
   const int64_t tile0 = (int64_t)blockIdx.x * kTile;
-  const int parts = gridDim.y, part = blockIdx.y;
   auto slot_of = [&](int64_t t) -> int64_t {
     if (t >= p.num_tokens) return -1;
     const int64_t slot = p.slot_mapping[t];
@@ -211,93 +262,146 @@ __global__ void __launch_bounds__(32 * kWarps) mrope_append_tile_kernel(const Mr
     raise_device_error(VASR_PA_DERR_SLOT_RANGE);
     return -1;
   };
-  {  // ---- q and k
+  const bool is_v = (int)blockIdx.y >= qk_parts;
+  const int part = is_v ? blockIdx.y - qk_parts : blockIdx.y, parts = is_v ? gridDim.y - qk_parts : qk_parts;
+  const int heads = is_v ? p.num_kv_heads : p.num_heads + p.num_kv_heads;
+  // prompts: a part has its heads [h0, h1) in shared memory; else they are dealt out
+  constexpr int kPartHeads = part_heads<T, D>(), kPitch = part_pitch<T, D>();
+  const int h0 = kPrompt ? part * kPartHeads : 0, h1 = kPrompt ? min(heads, h0 + kPartHeads) : heads;
+  extern __shared__ __align__(128) unsigned char rows[];
+  __shared__ __align__(8) uint64_t s_bar;
+  if constexpr (kPrompt) {
+    const uint32_t bar = smem_addr(&s_bar);
+    const int ntok = (int)min((int64_t)kTile, p.num_tokens - tile0);
+    const uint32_t bytes = (uint32_t)((h1 - h0) * D * (int)sizeof(T));
+    if (threadIdx.x == 0) {
+      mbar_init(bar, 1);
+      mbar_fence_init();
+      mbar_arrive_expect_tx(bar, ntok * bytes);
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < ntok)
+      bulk_g2s(smem_addr(rows) + threadIdx.x * kPitch,
+               static_cast<const T *>(p.qkv) + (tile0 + threadIdx.x) * p.qkv_token_stride +
+                   (int64_t)((is_v ? p.num_heads + p.num_kv_heads : 0) + h0) * D,
+               bytes, bar);
+  }
+  // false: the copies did not come (recorded); waited for once more, so that they do not outlive the CTA
+  auto rows_here = [&]() {
+    if constexpr (kPrompt) {
+      if (mbar_wait_bounded(smem_addr(&s_bar), 0)) return true;
+      mbar_wait_bounded(smem_addr(&s_bar), 0);
+      return false;
+    }
+    return true;
+  };
+  if (!is_v) {
     const int c = lane % L;
     const int64_t t = tile0 + (warp % kGroups) * kPerWarp + lane / L;
     const bool live = t < p.num_tokens;
     const int64_t tt = live ? t : p.num_tokens - 1;  // lanes past the end follow, for the shuffles
     const T *src = static_cast<const T *>(p.qkv) + tt * p.qkv_token_stride + c * kX;
+    const int step = kPrompt ? kHeadLanes : kHeadLanes * parts;
+    int h = h0 + warp / kGroups + (kPrompt ? 0 : kHeadLanes * part);
     const int64_t slot = slot_of(t);
-    Angles<kX> ang;
-    ang.load(p.rope, tt, c * kX);
-    const float k_scale = p.k_scale ? __ldg(p.k_scale) : 1.f;
-    auto head_range = [&](int first, int count, const T *weight, bool is_q) {
-      uint4 w0 = make_uint4(0, 0, 0, 0), w1 = w0;
-      if (weight) {
-        w0 = __ldg(reinterpret_cast<const uint4 *>(weight + c * kX));
-        w1 = __ldg(reinterpret_cast<const uint4 *>(weight + c * kX + D / 2));
-      }
-#pragma unroll 2
-      for (int h = warp / kGroups + kHeadLanes * part; h < count; h += kHeadLanes * parts) {
-        const T *row = src + (int64_t)(first + h) * D;
-        float a[kX], b[kX];
-        unpack_chunk<T>(__ldg(reinterpret_cast<const uint4 *>(row)), a);
-        unpack_chunk<T>(__ldg(reinterpret_cast<const uint4 *>(row + D / 2)), b);
-        if (weight) {
-          float ss = 0.f, wa[kX], wb[kX];
-#pragma unroll
-          for (int e = 0; e < kX; ++e) ss = fmaf(a[e], a[e], fmaf(b[e], b[e], ss));
-          const float inv = rsqrtf(warp_sum_xor(ss, L) / (float)D + p.eps);
-          unpack_chunk<T>(w0, wa);
-          unpack_chunk<T>(w1, wb);
-#pragma unroll
-          for (int e = 0; e < kX; ++e) {
-            a[e] *= inv * wa[e];
-            b[e] *= inv * wb[e];
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < kX; ++e) {
-          const float x = a[e];
-          a[e] = x * ang.c[e] - b[e] * ang.s[e];
-          b[e] = b[e] * ang.c[e] + x * ang.s[e];
-        }
-        if (is_q) {
-          if (live) {
-            T *q = static_cast<T *>(p.q_out) + (t * p.num_heads + h) * D + c * kX;
-            *reinterpret_cast<uint4 *>(q) = pack_chunk<T>(a);
-            *reinterpret_cast<uint4 *>(q + D / 2) = pack_chunk<T>(b);
-          }
-        } else if (slot >= 0) {
-          const int64_t page = (slot >> shift) * p.num_kv_heads + h;
-          const int off = (int)(slot & (p.block_size - 1));
-          auto place = [&](int d) {
-            return static_cast<TC *>(p.key_cache) + (((page * (D / kXc) + d / kXc) << shift) + off) * kXc + d % kXc;
-          };
-          store_key<TC, kX>(place(c * kX), a, k_scale);
-          store_key<TC, kX>(place(c * kX + D / 2), b, k_scale);
-          if (p.score_cache && c == 0) p.score_cache[(page << shift) + off] = 0.f;
-        }
+    auto load = [&](int head, uint4 (&r)[2]) {
+      if constexpr (kPrompt) {
+        const unsigned char *at = rows + (tt - tile0) * kPitch + ((head - h0) * D + c * kX) * (int)sizeof(T);
+        r[0] = *reinterpret_cast<const uint4 *>(at);
+        r[1] = *reinterpret_cast<const uint4 *>(at + D / 2 * (int)sizeof(T));
+      } else {
+        r[0] = __ldg(reinterpret_cast<const uint4 *>(src + (int64_t)head * D));
+        r[1] = __ldg(reinterpret_cast<const uint4 *>(src + (int64_t)head * D + D / 2));
       }
     };
-    head_range(0, p.num_heads, static_cast<const T *>(p.q_norm_weight), true);
-    head_range(p.num_heads, p.num_kv_heads, static_cast<const T *>(p.k_norm_weight), false);
-  }
-  {  // ---- v: item = (head, group of chunks), the tile's tokens across the lanes
-    constexpr int kChunks = 32 / kTile, kItems = C / kChunks;
-    const int64_t t = tile0 + lane % kTile;
-    const int cc = lane / kTile;
-    const int64_t slot = slot_of(t);
-    if (slot < 0) return;
-    const T *src = static_cast<const T *>(p.qkv) + t * p.qkv_token_stride + (int64_t)(p.num_heads + p.num_kv_heads) * D;
-    TC *dst = static_cast<TC *>(p.value_cache) + (((slot >> shift) * p.num_kv_heads * D) << shift) +
-              (slot & (p.block_size - 1));
-    const float v_scale = p.v_scale ? __ldg(p.v_scale) : 1.f;
-#pragma unroll 2
-    for (int i = warp + kWarps * part; i < p.num_kv_heads * kItems; i += kWarps * parts) {
-      const int d = (i * kChunks + cc) * kX;  // dim of the token's V row, over the heads
-      const uint4 raw = __ldg(reinterpret_cast<const uint4 *>(src + d));
-      TC *at = dst + ((int64_t)d << shift);
-      if constexpr (std::is_same<T, TC>::value) {
-        const T *e = reinterpret_cast<const T *>(&raw);
-#pragma unroll
-        for (int k = 0; k < kX; ++k) at[(int64_t)k << shift] = e[k];
-      } else {
-        float f[kX];
-        unpack_chunk<T>(raw, f);
-#pragma unroll
-        for (int k = 0; k < kX; ++k) at[(int64_t)k << shift] = __nv_fp8_e4m3(f[k] / v_scale);
+    uint4 raw[2], w[2];
+    if (!kPrompt && h < h1) load(h, raw);
+    Angles<kX> ang;
+    ang.load(p.rope, tt, c * kX);
+    if (!rows_here()) return;
+    const float k_scale = p.k_scale ? __ldg(p.k_scale) : 1.f;
+    const int64_t page0 = (slot >> shift) * p.num_kv_heads;
+    const int off = (int)(slot & (p.block_size - 1));
+    const T *weight = nullptr;
+    for (; h < h1; h += step) {
+      if constexpr (kPrompt) load(h, raw);
+      const bool is_q = h < p.num_heads;
+      const T *mine = static_cast<const T *>(is_q ? p.q_norm_weight : p.k_norm_weight);
+      if (mine != weight) {
+        weight = mine;
+        w[0] = __ldg(reinterpret_cast<const uint4 *>(weight + c * kX));
+        w[1] = __ldg(reinterpret_cast<const uint4 *>(weight + c * kX + D / 2));
       }
+      float a[kX], b[kX];
+      unpack_chunk<T>(raw[0], a);
+      unpack_chunk<T>(raw[1], b);
+      if (!kPrompt && h + step < h1) load(h + step, raw);  // while this row is worked on
+      if (weight) {
+        float s0 = 0.f, s1 = 0.f, wa[kX], wb[kX];
+#pragma unroll
+        for (int e = 0; e < kX; e += 2) {
+          fma2(s0, s1, a[e], a[e + 1], a[e], a[e + 1]);
+          fma2(s0, s1, b[e], b[e + 1], b[e], b[e + 1]);
+        }
+        const float inv = rsqrtf(warp_sum_xor(s0 + s1, L) / (float)D + p.eps);
+        unpack_chunk<T>(w[0], wa);
+        unpack_chunk<T>(w[1], wb);
+#pragma unroll
+        for (int e = 0; e < kX; e += 2) {
+          mul2(wa[e], wa[e + 1], wa[e], wa[e + 1], inv, inv);
+          mul2(wb[e], wb[e + 1], wb[e], wb[e + 1], inv, inv);
+          mul2(a[e], a[e + 1], a[e], a[e + 1], wa[e], wa[e + 1]);
+          mul2(b[e], b[e + 1], b[e], b[e + 1], wb[e], wb[e + 1]);
+        }
+      }
+      ang.turn(a, b);
+      if (is_q) {
+        if (live) {
+          T *q = static_cast<T *>(p.q_out) + (t * p.num_heads + h) * D + c * kX;
+          *reinterpret_cast<uint4 *>(q) = pack_chunk<T>(a);
+          *reinterpret_cast<uint4 *>(q + D / 2) = pack_chunk<T>(b);
+        }
+      } else if (slot >= 0) {
+        const int64_t page = page0 + h - p.num_heads;
+        auto place = [&](int d) {
+          return static_cast<TC *>(p.key_cache) + (((page * (D / kXc) + d / kXc) << shift) + off) * kXc + d % kXc;
+        };
+        store_key<TC, kX>(place(c * kX), a, k_scale);
+        store_key<TC, kX>(place(c * kX + D / 2), b, k_scale);
+        if (p.score_cache && c == 0) p.score_cache[(page << shift) + off] = 0.f;
+      }
+    }
+    return;
+  }
+  // ---- v: item = (head, group of chunks), the tile's tokens across the lanes
+  constexpr int kChunks = 32 / kTile, kItems = C / kChunks;
+  const int64_t t = tile0 + lane % kTile;
+  const int cc = lane / kTile;
+  const int64_t slot = slot_of(t);
+  if (!rows_here() || slot < 0) return;
+  const T *src = static_cast<const T *>(p.qkv) + t * p.qkv_token_stride + (int64_t)(p.num_heads + p.num_kv_heads) * D;
+  TC *dst = static_cast<TC *>(p.value_cache) + (((slot >> shift) * p.num_kv_heads * D) << shift) +
+            (slot & (p.block_size - 1));
+  const float v_scale = p.v_scale ? __ldg(p.v_scale) : 1.f;
+  const int step = kPrompt ? kCtaWarps : kCtaWarps * parts;
+#pragma unroll 4
+  for (int i = h0 * kItems + warp + (kPrompt ? 0 : kCtaWarps * part); i < h1 * kItems; i += step) {
+    const int d = (i * kChunks + cc) * kX;  // dim of the token's V row, over the heads
+    uint4 raw;
+    if constexpr (kPrompt)
+      raw = *reinterpret_cast<const uint4 *>(rows + lane % kTile * kPitch + (d - h0 * D) * (int)sizeof(T));
+    else
+      raw = __ldg(reinterpret_cast<const uint4 *>(src + d));
+    TC *at = dst + ((int64_t)d << shift);
+    if constexpr (std::is_same<T, TC>::value) {
+      const T *e = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+      for (int k = 0; k < kX; ++k) at[(int64_t)k << shift] = e[k];
+    } else {
+      float f[kX];
+      unpack_chunk<T>(raw, f);
+#pragma unroll
+      for (int k = 0; k < kX; ++k) at[(int64_t)k << shift] = __nv_fp8_e4m3(f[k] / v_scale);
     }
   }
 }
@@ -322,12 +426,7 @@ __global__ void __launch_bounds__(32 * kWarps) mrope_tile_kernel(const MropeArgs
     // plain loads: y may be x
     unpack_chunk<T>(*reinterpret_cast<const uint4 *>(x + h * p.x_head_stride), a);
     unpack_chunk<T>(*reinterpret_cast<const uint4 *>(x + h * p.x_head_stride + D / 2), b);
-#pragma unroll
-    for (int e = 0; e < kX; ++e) {
-      const float v = a[e];
-      a[e] = v * ang.c[e] - b[e] * ang.s[e];
-      b[e] = b[e] * ang.c[e] + v * ang.s[e];
-    }
+    ang.turn(a, b);
     *reinterpret_cast<uint4 *>(y + h * p.out_head_stride) = pack_chunk<T>(a);
     *reinterpret_cast<uint4 *>(y + h * p.out_head_stride + D / 2) = pack_chunk<T>(b);
   }
@@ -340,13 +439,26 @@ constexpr int kTargetCtas = 4 * 148;
 template <typename T, typename TC, int D, bool kPrompt>
 int launch_append_tile(const MropeAppendArgs &a, cudaStream_t s) {
   constexpr int kPerWarp = 32 / (D / Elem<T>::kX / 2);
-  constexpr int kTile = tile_tokens(kPerWarp, kPrompt), kHeadLanes = kWarps / (kTile / kPerWarp);
+  constexpr int kTile = tile_tokens(kPerWarp, kPrompt), kCtaWarps = tile_warps<T, D>(kPrompt);
+  constexpr int kHeadLanes = kCtaWarps / (kTile / kPerWarp);
   const int64_t tiles = (a.num_tokens + kTile - 1) / kTile;
-  const int most = (a.num_heads + kHeadLanes - 1) / kHeadLanes;
-  int64_t parts = kTargetCtas / tiles;
-  parts = parts < 1 ? 1 : parts > most ? most : parts;
-  if (tiles > 0x7fffffff || parts > 65535) return VASR_PA_EINVAL_SHAPE;
-  mrope_append_tile_kernel<T, TC, D, kPrompt><<<dim3((unsigned)tiles, (unsigned)parts), 32 * kWarps, 0, s>>>(a);
+  int64_t qk, v;
+  int smem = 0;
+  if (kPrompt) {
+    qk = (a.num_heads + a.num_kv_heads + part_heads<T, D>() - 1) / part_heads<T, D>();
+    v = (a.num_kv_heads + part_heads<T, D>() - 1) / part_heads<T, D>();
+    smem = kTile * part_pitch<T, D>();
+  } else {  // as many parts as give kTargetCtas, a part per row at most; V's share of them as its rows are of all
+    const int qk_most = (a.num_heads + a.num_kv_heads + kHeadLanes - 1) / kHeadLanes;
+    const int v_most = (a.num_kv_heads * (D / Elem<T>::kX) * kTile / 32 + kCtaWarps - 1) / kCtaWarps;
+    const int64_t parts = kTargetCtas / tiles > 2 ? kTargetCtas / tiles : 2;
+    v = parts * a.num_kv_heads / (a.num_heads + 2 * a.num_kv_heads);
+    v = v < 1 ? 1 : v > v_most ? v_most : v;
+    qk = parts - v;
+    qk = qk > qk_most ? qk_most : qk;
+  }
+  if (tiles > 0x7fffffff || qk + v > 65535) return VASR_PA_EINVAL_SHAPE;
+  mrope_append_tile_kernel<T, TC, D, kPrompt><<<dim3((unsigned)tiles, (unsigned)(qk + v)), 32 * kCtaWarps, smem, s>>>(a, (int)qk);
   return cudaPeekAtLastError() == cudaSuccess ? VASR_PA_OK : VASR_PA_ELAUNCH;
 }
 
@@ -369,7 +481,7 @@ int launch_tile(const MropeArgs &a, cudaStream_t s) {
 
 template <typename T, typename TC>
 int launch_append_tc(const MropeAppendArgs &a, cudaStream_t s) {
-  if (2 * a.rope.half == a.head_dim && aligned16(a.qkv) && (a.qkv_token_stride * (int64_t)sizeof(T)) % 16 == 0 &&
+  if (2 * a.rope.half == a.head_dim && aligned16(a.rope.cos_table) && aligned16(a.rope.sin_table) && aligned16(a.qkv) && (a.qkv_token_stride * (int64_t)sizeof(T)) % 16 == 0 &&
       aligned16(a.q_out) && aligned16(a.q_norm_weight) && aligned16(a.k_norm_weight)) {
     switch (a.head_dim) {
       case 64: return launch_append_d<T, TC, 64>(a, s);
@@ -394,7 +506,7 @@ int launch_append_t(const MropeAppendArgs &a, cudaStream_t s) {
 template <typename T>
 int launch_rows_t(const MropeArgs &a, cudaStream_t s) {
   auto whole = [](int64_t stride) { return stride * (int64_t)sizeof(T) % 16 == 0; };
-  if (2 * a.rope.half == a.head_dim && aligned16(a.x) && aligned16(a.out) && whole(a.x_token_stride) &&
+  if (2 * a.rope.half == a.head_dim && aligned16(a.rope.cos_table) && aligned16(a.rope.sin_table) && aligned16(a.x) && aligned16(a.out) && whole(a.x_token_stride) &&
       whole(a.x_head_stride) && whole(a.out_token_stride) && whole(a.out_head_stride)) {
     switch (a.head_dim) {
       case 64: return launch_tile<T, 64>(a, s);
