@@ -271,6 +271,7 @@ struct VerifyArgs {
   // filled by launch_verify
   int row_chunks;
   void *stats;
+  void *verdicts;
   void *bests;
   uint32_t *counters;
 };

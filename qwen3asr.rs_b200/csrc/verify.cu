@@ -12,14 +12,17 @@
 // long f32 sum. T = 0: accept while x_i is the argmax of row i, then take row
 // n's argmax. Lowest index on equal values; NaN logits count as -inf.
 //
-// Two launches. The first gives every chunk of every row its maximum and its
-// sum of exp((x - max) / T) in one pass: a thread keeps its logits in
-// registers between the maximum and the sum. The second, a programmatic
-// dependent of the first, has a CTA per chunk of a sequence's vocabulary: it
-// loads its noise and the drafts' logits early, joins the rows' chunks and
-// decides on its own copy (a few hundred bytes), runs the race over its chunk
-// of row n, and the last CTA of the sequence takes the winner. Only the row
-// that is drawn from is read twice, the second time from L2.
+// Three launches, each a programmatic dependent of the one before. The first
+// gives every chunk of every row its maximum and its sum of exp((x - max) / T)
+// in one pass over the logits, which a thread keeps in registers between its
+// maximum and its sum. The second, a CTA per sequence, joins the chunks and
+// writes the verdict (n, row n's maximum and sum); a counter that elects the
+// sequence's last CTA of the first launch instead made every CTA of that
+// launch wait for its own atomic (40 against 30 us at 64 x 5 rows of 151936).
+// The third runs the race over row n, a CTA per chunk of the vocabulary: it
+// has its noise in registers by the time the verdict is there, and the last
+// CTA of a sequence takes the winner. Only the row that is drawn from is read
+// twice, the second time from L2.
 #include <type_traits>
 
 #include "common.cuh"
@@ -28,9 +31,11 @@
 namespace vasr {
 namespace {
 
-constexpr int kRowElems = 32;   // logits a thread of the first launch keeps in registers
-constexpr int kEmitElems = 16;  // logits, drafter's values and noise each of the second's (80 registers)
+constexpr int kRowElems = 64;   // logits a thread of the first launch keeps (32 for f32: 16 vectors)
+constexpr int kEmitElems = 16;  // logits, drafter's values and noise each that one of the second's does
 constexpr int kMaxThreads = 256;
+template <typename T>
+constexpr int row_elems() { return sizeof(T) == 4 ? kRowElems / 2 : kRowElems; }
 
 // One chunk of a row: its maximum (and, for greedy rows, the first place of
 // it) and sum over the chunk of exp((x - max) / T).
@@ -39,6 +44,14 @@ struct ChunkStat {
   float sum;
   uint32_t arg;
   uint32_t pad;
+};
+
+// What the second launch found out about a sequence.
+struct Verdict {
+  int n;        // accepted drafts
+  float max;    // of row n
+  float inv;    // 1 / its sum
+  int32_t drawn;  // the race is to be run (else the tokens are written already)
 };
 
 // (value, index): larger value first, then lower index.
@@ -97,19 +110,24 @@ struct Held {
 #pragma unroll
     for (int k = 0; k < kGroups; ++k) {
       const int j = (tid + k * threads) * kGroup;
-      if (aligned && j + kGroup <= len) {
+      if (aligned && (k + 1) * threads * kGroup <= len) {  // the whole CTA's groups
 #pragma unroll
         for (int v = 0; v < kVecs; ++v) raw[k][v] = __ldg(reinterpret_cast<const uint4 *>(row + j) + v);
       } else {
 #pragma unroll
         for (int v = 0; v < kVecs; ++v) {
-          T e[kVec];
+          raw[k][v] = make_uint4(0, 0, 0, 0);
+          if (aligned && j + kGroup <= len) {
+            raw[k][v] = __ldg(reinterpret_cast<const uint4 *>(row + j) + v);
+          } else if (j < len) {
+            T e[kVec];
 #pragma unroll
-          for (int i = 0; i < kVec; ++i) {
-            const int at = j + v * kVec + i;
-            e[i] = at < len ? row[at] : Elem<T>::from_f32(0.f);
+            for (int i = 0; i < kVec; ++i) {
+              const int at = j + v * kVec + i;
+              e[i] = at < len ? row[at] : Elem<T>::from_f32(0.f);
+            }
+            raw[k][v] = *reinterpret_cast<const uint4 *>(e);
           }
-          raw[k][v] = *reinterpret_cast<const uint4 *>(e);
         }
       }
     }
@@ -141,248 +159,273 @@ struct Held {
   }
 };
 
-// The guarded forms for a chunk's rest (fewer than 8 elements of a group) and
-// for logits that are not finite.
+// f(value, index) for the thread's elements of group k that lie in the chunk
+// and are not NaN; groups past a chunk's end have none.
 template <typename T, int kGroups, typename F>
-__device__ __forceinline__ void each_guarded(const Held<T, kGroups> &x, int len, int tid, int threads, F f) {
-  for (int k = 0; k < kGroups; ++k) {
-    float v[kGroup];
-    x.group(k, v);
-    const int j = (tid + k * threads) * kGroup;
+__device__ __forceinline__ void each_of_group(const Held<T, kGroups> &x, int k, int len, int tid, int threads, F f) {
+  const int j = (tid + k * threads) * kGroup;
+  if (j >= len) return;
+  float v[kGroup];
+  x.group(k, v);
 #pragma unroll
-    for (int i = 0; i < kGroup; ++i)
-      if (j + i < len && v[i] == v[i]) f(v[i], j + i);
-  }
+  for (int i = 0; i < kGroup; ++i)
+    if (j + i < len && v[i] == v[i]) f(v[i], j + i);
 }
 
+// grid = (chunk, row, sequence)
 template <typename T>
 __global__ void __launch_bounds__(kMaxThreads) verify_rows_kernel(const VerifyArgs p) {
   pdl_launch_dependents();
-  constexpr int kGroups = kRowElems / kGroup;
+  constexpr int kGroups = row_elems<T>() / kGroup;
+  __shared__ float2 part[kMaxThreads / 32];
+  __shared__ uint32_t s_arg;
   const int chunk = blockIdx.x, i = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, threads = blockDim.x;
+  const int warp = tid >> 5, lane = tid & 31, warps = threads >> 5;
   if (i > drafts_of(p, b)) return;
-  const int size = threads * kRowElems;
+  const float t = temperature_of(p, b);
+  const int size = threads * row_elems<T>();
   const int64_t lo = (int64_t)chunk * size;
   const int len = (int)min((int64_t)size, p.vocab - lo);
-  const T *row = static_cast<const T *>(p.logits) + b * p.logits_seq_stride + i * p.logits_row_stride + lo;
   Held<T, kGroups> x;
-  x.load(row, len, tid, threads);
-  const float t = temperature_of(p, b);
-  float m = -INFINITY;
-  if (len == size) {
+  x.load(static_cast<const T *>(p.logits) + b * p.logits_seq_stride + i * p.logits_row_stride + lo, len, tid, threads);
+  // the thread's own maximum and sum, then the warp's, then the chunk's
+  const int whole = len / (threads * kGroup);  // groups that all threads have
+  float m = -INFINITY, sum = 0.f;
 #pragma unroll
-    for (int k = 0; k < kGroups; ++k) m = fmaxf(m, x.group_max(k));
-  } else {
-    each_guarded(x, len, tid, threads, [&](float v, int) { m = fmaxf(m, v); });
+  for (int g = 0; g < kGroups; ++g) {
+    if (g < whole) m = fmaxf(m, x.group_max(g));
+    else each_of_group(x, g, len, tid, threads, [&](float v, int) { m = fmaxf(m, v); });
   }
-  __shared__ float part[kMaxThreads / 32];
-  __shared__ uint32_t s_arg;
-  const int warps = threads >> 5;
-  m = warp_max_xor(m, 32);
-  if ((tid & 31) == 0) part[tid >> 5] = m;
-  if (tid == 0) s_arg = kNone;
-  __syncthreads();
-  for (int w = 0; w < warps; ++w) m = fmaxf(m, part[w]);
-  __syncthreads();
-  float sum = 0.f;
-  if (t > 0.f) {
-    const float c = kLog2e / t;
-    if (m > -INFINITY) {
-      if (len == size) {
+  const float c = kLog2e / t;
+  if (t > 0.f && m > -INFINITY) {
 #pragma unroll
-        for (int k = 0; k < kGroups; ++k) {
-          float v[kGroup];
-          x.group(k, v);
+    for (int g = 0; g < kGroups; ++g) {
+      if (g < whole) {
+        float v[kGroup];
+        x.group(g, v);
 #pragma unroll
-          for (int e = 0; e < kGroup; ++e) sum += plain_weight(v[e], m, c);
-        }
-      }
-      if (len != size || !(sum == sum)) {
-        sum = 0.f;
-        each_guarded(x, len, tid, threads, [&](float v, int) { sum += weight_of(v, m, c); });
+        for (int e = 0; e < kGroup; ++e) sum += plain_weight(v[e], m, c);
+      } else {
+        each_of_group(x, g, len, tid, threads, [&](float v, int) { sum += weight_of(v, m, c); });
       }
     }
-    sum = warp_sum_xor(sum, 32);
-    if ((tid & 31) == 0) part[tid >> 5] = sum;
-    __syncthreads();
-    sum = 0.f;
-    for (int w = 0; w < warps; ++w) sum += part[w];
-  } else {
+    if (!(sum == sum)) {  // an infinite maximum or a NaN among the logits
+      sum = 0.f;
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g)
+        each_of_group(x, g, len, tid, threads, [&](float v, int) { sum += weight_of(v, m, c); });
+    }
+  }
+  const float wm = warp_max_xor(m, 32);
+  if (t > 0.f) sum = warp_sum_xor(m > -INFINITY ? sum * weight_of(m, wm, c) : 0.f, 32);
+  if (lane == 0) part[warp] = make_float2(wm, sum);
+  if (tid == 0) s_arg = kNone;
+  __syncthreads();
+  const bool greedy = !(t > 0.f);
+  if (!greedy && warp != 0) return;
+  const float2 mine = part[lane < warps ? lane : 0];
+  const float cm = warp_max_xor(mine.x, 32);
+  if (greedy) {  // the first place of the maximum
     uint32_t first = kNone;
-    each_guarded(x, len, tid, threads, [&](float v, int j) {
-      if (v == m) first = min(first, (uint32_t)j);
-    });
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g)
+      each_of_group(x, g, len, tid, threads, [&](float v, int j) {
+        if (v == cm) first = min(first, (uint32_t)j);
+      });
     if (first != kNone) atomicMin(&s_arg, first);
     __syncthreads();
+  } else {
+    sum = warp_sum_xor(lane < warps && mine.y != 0.f ? mine.y * weight_of(mine.x, cm, c) : 0.f, 32);
   }
-  if (tid == 0) {
-    ChunkStat *out = static_cast<ChunkStat *>(p.stats);
-    out[((int64_t)b * (p.num_drafts + 1) + i) * p.row_chunks + chunk] =
-        ChunkStat{m, sum, s_arg != kNone ? (uint32_t)lo + s_arg : 0u, 0u};
-  }
+  if (tid == 0)
+    static_cast<ChunkStat *>(p.stats)[((int64_t)b * (p.num_drafts + 1) + i) * gridDim.x + chunk] =
+        ChunkStat{cm, sum, s_arg != kNone ? (uint32_t)lo + s_arg : 0u, 0u};
 }
 
 // A whole row from its chunks, by one warp.
 __device__ __forceinline__ ChunkStat join_chunks(const VerifyArgs &p, int64_t row, float t) {
-  const int lane = threadIdx.x & 31;
-  const ChunkStat *s = static_cast<const ChunkStat *>(p.stats) + row * p.row_chunks;
+  const int lane = threadIdx.x & 31, chunks = p.row_chunks;
+  const float4 *s = static_cast<const float4 *>(p.stats) + row * chunks;
   Best top{-INFINITY, kNone};
-  for (int c = lane; c < p.row_chunks; c += 32)
-    if (s[c].max > -INFINITY) top = better(top, Best{s[c].max, s[c].arg});
+  for (int c = lane; c < chunks; c += 32) {
+    const float4 v = s[c];
+    if (v.x > -INFINITY) top = better(top, Best{v.x, __float_as_uint(v.z)});
+  }
   top = warp_best(top);
   float sum = 0.f;
   if (t > 0.f && top.v > -INFINITY) {
     const float k = kLog2e / t;
-    for (int c = lane; c < p.row_chunks; c += 32)
-      if (s[c].sum != 0.f) sum = fmaf(s[c].sum, weight_of(s[c].max, top.v, k), sum);
+    for (int c = lane; c < chunks; c += 32) {
+      const float4 v = s[c];
+      if (v.y != 0.f) sum = fmaf(v.y, weight_of(v.x, top.v, k), sum);
+    }
     sum = warp_sum_xor(sum, 32);
   }
   return ChunkStat{top.v, sum, top.i != kNone ? top.i : 0u, 0u};
 }
 
+// One CTA per sequence: every row's sum, then the verdict.
 template <typename T, typename TQ>
-__global__ void __launch_bounds__(kMaxThreads, 4) verify_emit_kernel(const VerifyArgs p) {
+__global__ void __launch_bounds__(kMaxThreads) verify_verdict_kernel(const VerifyArgs p) {
+  pdl_launch_dependents();
   extern __shared__ ChunkStat s_row[];  // [num_drafts + 1]
   __shared__ int s_fail;
-  __shared__ Best part[kMaxThreads / 32];
-  __shared__ uint32_t s_last;
-  const int chunk = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, threads = blockDim.x;
-  const int warp = tid >> 5, lane = tid & 31, warps = threads >> 5;
+  const int b = blockIdx.x, tid = threadIdx.x, threads = blockDim.x, warp = tid >> 5, lane = tid & 31;
   const int k = drafts_of(p, b);
   const float t = temperature_of(p, b);
   const T *rows = static_cast<const T *>(p.logits) + b * p.logits_seq_stride;
-  const TQ *probs = p.draft_probs ? static_cast<const TQ *>(p.draft_probs) + b * p.probs_seq_stride : nullptr;
   const int32_t *drafts = p.draft_tokens + (int64_t)b * p.num_drafts;
-  constexpr int kGroups = kEmitElems / kGroup;
-  const int size = threads * kEmitElems;
-  const int64_t lo = (int64_t)chunk * size;
-  const int len = (int)min((int64_t)size, p.vocab - lo);
-  if (tid == 0) s_fail = k;
-  // inputs that the first launch does not write
-  Held<float, kGroups> race;
-  if (t > 0.f) race.load(p.race + b * p.race_seq_stride + lo, len, tid, threads);
+  const TQ *probs = p.draft_probs ? static_cast<const TQ *>(p.draft_probs) + b * p.probs_seq_stride : nullptr;
+  // a draft's target logit, drafter's probability and uniform (inputs: read ahead of the first launch's end)
+  auto draft = [&](int r, int32_t &x, float &logit, float &q, float &u) {
+    x = drafts[r];
+    if (x < 0 || x >= p.vocab) x = -1;
+    logit = x >= 0 ? Elem<T>::to_f32(rows[r * p.logits_row_stride + x]) : -INFINITY;
+    q = probs && x >= 0 ? Elem<TQ>::to_f32(probs[r * p.probs_row_stride + x]) : 1.f;
+    u = t > 0.f ? p.uniform[(int64_t)b * p.num_drafts + r] : 0.f;
+  };
   int32_t x0 = -1;
-  float logit0 = -INFINITY, q0 = 1.f, u0 = 0.f;
-  if (tid < k) {
-    x0 = drafts[tid];
-    if (x0 >= 0 && x0 < p.vocab) {
-      logit0 = fmaxf(Elem<T>::to_f32(rows[tid * p.logits_row_stride + x0]), -INFINITY);
-      if (probs) q0 = Elem<TQ>::to_f32(probs[tid * p.probs_row_stride + x0]);
-    }
-    if (t > 0.f) u0 = p.uniform[(int64_t)b * p.num_drafts + tid];
-  }
+  float logit0 = 0.f, q0 = 0.f, u0 = 0.f;
+  if (tid < k) draft(tid, x0, logit0, q0, u0);
+  if (tid == 0) s_fail = k;
   pdl_wait();
-  for (int i = warp; i <= k; i += warps) {
-    const ChunkStat s = join_chunks(p, (int64_t)b * (p.num_drafts + 1) + i, t);
-    if (lane == 0) s_row[i] = s;
+  for (int r = warp; r <= k; r += threads >> 5) {
+    const ChunkStat s = join_chunks(p, (int64_t)b * (p.num_drafts + 1) + r, t);
+    if (lane == 0) s_row[r] = s;
   }
   __syncthreads();
-  const float c = t > 0.f ? kLog2e / t : 0.f;
-  for (int i = tid; i < k; i += threads) {
+  for (int r = tid; r < k; r += threads) {
     int32_t x = x0;
     float logit = logit0, q = q0, u = u0;
-    if (i != tid) {
-      x = drafts[i];
-      logit = -INFINITY;
-      q = 1.f;
-      u = t > 0.f ? p.uniform[(int64_t)b * p.num_drafts + i] : 0.f;
-      if (x >= 0 && x < p.vocab) {
-        logit = fmaxf(Elem<T>::to_f32(rows[i * p.logits_row_stride + x]), -INFINITY);
-        if (probs) q = Elem<TQ>::to_f32(probs[i * p.probs_row_stride + x]);
-      }
-    }
-    const ChunkStat s = s_row[i];
-    bool ok = x >= 0 && x < p.vocab && s.max > -INFINITY;
-    if (ok) ok = t > 0.f ? u * q < weight_of(logit, s.max, c) / s.sum : (uint32_t)x == s.arg;
-    if (!ok) atomicMin(&s_fail, i);
+    if (r != tid) draft(r, x, logit, q, u);
+    const ChunkStat s = s_row[r];
+    bool ok = x >= 0 && s.max > -INFINITY;
+    if (ok) ok = t > 0.f ? u * q < weight_of(logit, s.max, kLog2e / t) / s.sum : (uint32_t)x == s.arg;
+    if (!ok) atomicMin(&s_fail, r);
   }
   __syncthreads();
   const int n = s_fail;
   const ChunkStat s = s_row[n];
-  const T *row = rows + n * p.logits_row_stride;
-  const int64_t failed = n < k ? (int64_t)drafts[n] : -1;
-  const TQ *qrow = probs && n < k ? probs + n * p.probs_row_stride : nullptr;
   const bool drawn = t > 0.f && s.max > -INFINITY;
-  uint32_t next = s.arg;
-  if (drawn) {
-    // ---- the race over this chunk. The quotient takes one reciprocal
-    // instruction (1 ulp); only r / e > 0 can win, so NaN and r <= 0 drop out.
-    Held<T, kGroups> x;
-    x.load(row + lo, len, tid, threads);
-    Held<TQ, kGroups> q;
-    if (qrow) q.load(qrow + lo, len, tid, threads);
-    const float inv = 1.f / s.sum;
-    const bool finite = s.max < INFINITY && c < INFINITY;
-    const int skip = failed >= lo && failed < lo + len && !qrow ? (int)(failed - lo) : -1;
-    Best best{0.f, kNone};
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-      const int j = (tid + g * threads) * kGroup;
-      float w[kGroup], e[kGroup], qv[kGroup];
-      x.group(g, w);
-      race.group(g, e);
-      if (qrow) {
-        q.group(g, qv);
-      } else {
-#pragma unroll
-        for (int i = 0; i < kGroup; ++i) qv[i] = 0.f;
-      }
-#pragma unroll
-      for (int i = 0; i < kGroup; ++i) {
-        const float pw = finite ? plain_weight(w[i], s.max, c) : weight_of(w[i], s.max, c);
-        float a = fmaf(pw, inv, -qv[i]) * rcp_approx(e[i]);
-        if (j + i >= len || j + i == skip) a = 0.f;
-        if (a > best.v) best = Best{a, (uint32_t)(j + i)};
-      }
-    }
-    if (best.i != kNone) best.i += (uint32_t)lo;
-    best = warp_best(best);
-    if (lane == 0) part[warp] = best;
-    __syncthreads();
-    if (tid == 0) {
-      for (int w = 1; w < warps; ++w) best = better(best, part[w]);
-      Best *slots = static_cast<Best *>(p.bests) + (int64_t)b * gridDim.x;
-      slots[chunk] = best;
-      __threadfence();
-      s_last = atomicAdd(p.counters + b, 1u) == gridDim.x - 1;
-      __threadfence();
-    }
-    __syncthreads();
-    if (!s_last) return;
-    // ---- the sequence's last CTA: the winner over all chunks
-    best = Best{0.f, kNone};
-    const Best *slots = static_cast<const Best *>(p.bests) + (int64_t)b * gridDim.x;
-    for (int i = tid; i < (int)gridDim.x; i += threads) best = better(best, Best{__ldcg(&slots[i].v), __ldcg(&slots[i].i)});
-    best = warp_best(best);
-    if (lane == 0) part[warp] = best;
-    __syncthreads();
-    best = part[0];
-    for (int w = 1; w < warps; ++w) best = better(best, part[w]);
-    if (best.i == kNone) {  // r is 0 everywhere (the drafter covers the target): draw from p
-      __syncthreads();
-      const float *noise = p.race + b * p.race_seq_stride;
-      for (int64_t v = tid; v < p.vocab; v += threads) {
-        const float a = weight_of(Elem<T>::to_f32(row[v]), s.max, c) * inv * rcp_approx(noise[v]);
-        if (a > best.v) best = Best{a, (uint32_t)v};
-      }
-      best = warp_best(best);
-      if (lane == 0) part[warp] = best;
-      __syncthreads();
-      best = part[0];
-      for (int w = 1; w < warps; ++w) best = better(best, part[w]);
-    }
-    next = best.i != kNone ? best.i : 0u;  // all noise NaN
-    if (tid == 0) p.counters[b] = 0u;
-  } else if (chunk != 0) {
-    return;
+  if (tid == 0) {
+    static_cast<Verdict *>(p.verdicts)[b] = Verdict{n, s.max, 1.f / s.sum, drawn};
+    p.num_accepted[b] = n;
   }
-  int32_t *out = p.out_tokens + (int64_t)b * (p.num_drafts + 1);
-  for (int i = tid; i <= p.num_drafts; i += threads) out[i] = i < n ? drafts[i] : i == n ? (int32_t)next : -1;
-  if (tid == 0) p.num_accepted[b] = n;
+  int32_t *out = p.out_tokens + (int64_t)b * (p.num_drafts + 1);  // all but the drawn token
+  for (int r = tid; r <= p.num_drafts; r += threads)
+    if (r != n || !drawn) out[r] = r < n ? drafts[r] : r == n ? (int32_t)s.arg : -1;
 }
 
-// 8192 logits a chunk (256 threads); calls whose chunks would not fill the SMs
-// take chunks of 2048 (64 threads), which cost more CTAs per byte.
+// grid = (chunk, sequence)
+template <typename T, typename TQ>
+__global__ void __launch_bounds__(kMaxThreads, 4) verify_emit_kernel(const VerifyArgs p) {
+  constexpr int kGroups = kEmitElems / kGroup;
+  __shared__ Best part[kMaxThreads / 32];
+  const int chunk = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, threads = blockDim.x;
+  const int warp = tid >> 5, lane = tid & 31, warps = threads >> 5;
+  const float t = temperature_of(p, b);
+  const int size = threads * kEmitElems;
+  const int64_t lo = (int64_t)chunk * size;
+  const int len = (int)min((int64_t)size, p.vocab - lo);
+  // inputs come early, while the launches before still run
+  Held<float, kGroups> race;
+  if (t > 0.f) race.load(p.race + b * p.race_seq_stride + lo, len, tid, threads);
+  const int k = drafts_of(p, b);
+  pdl_wait();
+  const float4 raw = __ldcg(static_cast<const float4 *>(p.verdicts) + b);
+  const Verdict s{__float_as_int(raw.x), raw.y, raw.z, __float_as_int(raw.w)};
+  if (!s.drawn) return;
+  const float c = kLog2e / t;
+  const T *row = static_cast<const T *>(p.logits) + b * p.logits_seq_stride + s.n * p.logits_row_stride;
+  // ---- the race over this chunk. The quotient takes one reciprocal
+  // instruction (1 ulp); only r / e > 0 can win, so NaN and r <= 0 drop out.
+  Held<T, kGroups> x;
+  x.load(row + lo, len, tid, threads);
+  const bool with_q = p.draft_probs && s.n < k;
+  Held<TQ, kGroups> q;
+  if (with_q)
+    q.load(static_cast<const TQ *>(p.draft_probs) + b * p.probs_seq_stride + s.n * p.probs_row_stride + lo, len, tid,
+           threads);
+  int skip = -1;  // a failed draft that the drafter was certain of
+  if (s.n < k && !with_q) {
+    const int64_t failed = (int64_t)p.draft_tokens[(int64_t)b * p.num_drafts + s.n] - lo;
+    if (failed >= 0 && failed < len) skip = (int)failed;
+  }
+  const bool finite = s.max < INFINITY && c < INFINITY;
+  float top = 0.f;
+  int place = -1;  // g * 8 + i of the winner
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) {
+    const int j = (tid + g * threads) * kGroup;
+    float w[kGroup], e[kGroup], qv[kGroup];
+    x.group(g, w);
+    race.group(g, e);
+    if (with_q) {
+      q.group(g, qv);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kGroup; ++i) qv[i] = 0.f;
+    }
+    if (finite && j + kGroup <= len && (skip < j || skip >= j + kGroup)) {
+#pragma unroll
+      for (int i = 0; i < kGroup; ++i) {
+        const float a = fmaf(plain_weight(w[i], s.max, c), s.inv, -qv[i]) * rcp_approx(e[i]);
+        if (a > top) {
+          top = a;
+          place = g * kGroup + i;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kGroup; ++i) {
+        const float a = fmaf(weight_of(w[i], s.max, c), s.inv, -qv[i]) * rcp_approx(e[i]);
+        if (a > top && j + i < len && j + i != skip) {
+          top = a;
+          place = g * kGroup + i;
+        }
+      }
+    }
+  }
+  Best best{top, kNone};
+  if (place >= 0) best.i = (uint32_t)(lo + (tid + place / kGroup * threads) * kGroup + place % kGroup);
+  best = warp_best(best);
+  if (lane == 0) part[warp] = best;
+  __syncthreads();
+  if (warp != 0) return;
+  best = lane < warps ? part[lane] : Best{0.f, kNone};
+  best = warp_best(best);
+  uint64_t *slots = static_cast<uint64_t *>(p.bests) + (int64_t)b * gridDim.x;
+  uint32_t last = 0;
+  if (lane == 0) {
+    slots[chunk] = (uint64_t)__float_as_uint(best.v) << 32 | best.i;
+    __threadfence();
+    last = atomicAdd(p.counters + b, 1u) == gridDim.x - 1;
+    __threadfence();
+  }
+  if (!__shfl_sync(0xffffffffu, last, 0)) return;
+  // ---- the sequence's last CTA: the winner over all chunks
+  best = Best{0.f, kNone};
+  for (int i = lane; i < (int)gridDim.x; i += 32) {
+    const uint64_t v = __ldcg(reinterpret_cast<const unsigned long long *>(slots) + i);
+    best = better(best, Best{__uint_as_float((uint32_t)(v >> 32)), (uint32_t)v});
+  }
+  best = warp_best(best);
+  if (best.i == kNone) {  // r is 0 everywhere (the drafter covers the target): draw from p
+    const float *noise = p.race + b * p.race_seq_stride;
+    for (int64_t v = lane; v < p.vocab; v += 32) {
+      const float a = weight_of(Elem<T>::to_f32(row[v]), s.max, c) * s.inv * rcp_approx(noise[v]);
+      if (a > best.v) best = Best{a, (uint32_t)v};
+    }
+    best = warp_best(best);
+  }
+  if (lane == 0) {
+    p.out_tokens[(int64_t)b * (p.num_drafts + 1) + s.n] = best.i != kNone ? (int32_t)best.i : 0;  // 0: all noise NaN
+    p.counters[b] = 0u;
+  }
+}
+
+// CTAs of 256 threads; calls whose chunks would not fill the SMs take CTAs of
+// 64, which cost more reductions per byte.
 int chunk_threads(int num_seqs, int num_drafts, int64_t vocab) {
   const int64_t ctas = (int64_t)num_seqs * (num_drafts + 1) * ((vocab + 8191) / 8192);
   return ctas >= 2 * 148 ? 256 : 64;
@@ -390,41 +433,48 @@ int chunk_threads(int num_seqs, int num_drafts, int64_t vocab) {
 
 struct VerifyLayout {
   int threads, row_chunks, emit_chunks;
-  size_t off_stats, off_bests, total;
+  size_t off_stats, off_verdicts, off_bests, total;
 };
 constexpr size_t kCounterBytes = 65536 * sizeof(uint32_t);  // one per sequence, left at zero
-VerifyLayout verify_layout(int num_seqs, int num_drafts, int64_t vocab) {
+VerifyLayout verify_layout(int num_seqs, int num_drafts, int64_t vocab, int row_elems) {
   VerifyLayout l;
   l.threads = chunk_threads(num_seqs, num_drafts, vocab);
   auto chunks = [&](int elems) { return (int)((vocab + l.threads * elems - 1) / (l.threads * elems)); };
-  l.row_chunks = chunks(kRowElems);
+  l.row_chunks = chunks(row_elems);
   l.emit_chunks = chunks(kEmitElems);
   l.off_stats = kCounterBytes;
-  l.off_bests = l.off_stats + (size_t)num_seqs * (num_drafts + 1) * l.row_chunks * sizeof(ChunkStat);
-  l.total = l.off_bests + (size_t)num_seqs * l.emit_chunks * sizeof(Best);
+  l.off_verdicts = l.off_stats + (size_t)num_seqs * (num_drafts + 1) * l.row_chunks * sizeof(ChunkStat);
+  l.off_bests = l.off_verdicts + (size_t)num_seqs * sizeof(Verdict);
+  l.total = l.off_bests + (size_t)num_seqs * l.emit_chunks * sizeof(uint64_t);
   return l;
 }
 
 template <typename T, typename TQ>
 int launch_verify_tq(VerifyArgs a, cudaStream_t s) {
-  const VerifyLayout l = verify_layout(a.num_seqs, a.num_drafts, a.vocab);
+  const VerifyLayout l = verify_layout(a.num_seqs, a.num_drafts, a.vocab, row_elems<T>());
   unsigned char *ws = static_cast<unsigned char *>(a.workspace);
   a.counters = reinterpret_cast<uint32_t *>(ws);
   a.stats = ws + l.off_stats;
+  a.verdicts = ws + l.off_verdicts;
   a.bests = ws + l.off_bests;
   a.row_chunks = l.row_chunks;
   verify_rows_kernel<T><<<dim3((unsigned)l.row_chunks, (unsigned)a.num_drafts + 1, (unsigned)a.num_seqs),
                           (unsigned)l.threads, 0, s>>>(a);
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)l.emit_chunks, (unsigned)a.num_seqs);
-  cfg.blockDim = dim3((unsigned)l.threads);
-  cfg.dynamicSmemBytes = (size_t)(a.num_drafts + 1) * sizeof(ChunkStat);
-  cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  cfg.stream = s;
+  const int row_warps = a.num_drafts + 1 < kMaxThreads / 32 ? a.num_drafts + 1 : kMaxThreads / 32;
+  cfg.gridDim = dim3((unsigned)a.num_seqs);
+  cfg.blockDim = dim3((unsigned)row_warps * 32);
+  cfg.dynamicSmemBytes = (size_t)(a.num_drafts + 1) * sizeof(ChunkStat);
+  if (cudaLaunchKernelEx(&cfg, verify_verdict_kernel<T, TQ>, a) != cudaSuccess) return VASR_PA_ELAUNCH;
+  cfg.gridDim = dim3((unsigned)l.emit_chunks, (unsigned)a.num_seqs);
+  cfg.blockDim = dim3((unsigned)l.threads);
+  cfg.dynamicSmemBytes = 0;
   return cudaLaunchKernelEx(&cfg, verify_emit_kernel<T, TQ>, a) == cudaSuccess ? VASR_PA_OK : VASR_PA_ELAUNCH;
 }
 
@@ -441,7 +491,7 @@ int launch_verify_t(const VerifyArgs &a, cudaStream_t s) {
 }  // namespace
 
 size_t verify_workspace_bytes(int num_seqs, int num_drafts, int64_t vocab) {
-  return verify_layout(num_seqs, num_drafts, vocab).total;
+  return verify_layout(num_seqs, num_drafts, vocab, kRowElems / 2).total;  // the most chunks of any type
 }
 
 int launch_verify(const VerifyArgs &a, cudaStream_t s) {
