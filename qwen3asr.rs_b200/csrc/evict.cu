@@ -8,19 +8,24 @@
 // its own set, which the page layout allows because a block holds each head's
 // tokens apart.
 //
-// Selection is a radix select over order-preserving keys of the scores; the
-// move copies bits. In place, token r of the result comes from an index >= r,
-// so places filled in ascending tiles never overwrite a token that is still
-// needed, as long as a tile is read before it or a later one is written: each
-// CTA moves one slice of the head dimension of one (sequence, head) that way.
+// Selection is a radix select over order-preserving keys of the scores, which
+// a CTA per (sequence, kv head) keeps in shared memory; the move copies bits,
+// bound by memory: it reads every 32-byte sector that holds a kept token and
+// writes the kept ones. In place, token r of the result comes from an index
+// >= r, so places filled in ascending tiles never overwrite a token that is
+// still needed, as long as a tile is read before it or a later one is written:
+// a CTA moves its slices of the head dimension of one (sequence, head) that way.
 #include "common.cuh"
 #include "launch.h"
 
 namespace vasr {
 namespace {
 
-constexpr int kSelectThreads = 256;
+constexpr int kSelectThreads = 512;
+constexpr int kSelectWarps = kSelectThreads / 32;
 constexpr int kMoveThreads = 256;
+constexpr int kMoveMostThreads = 1024;
+constexpr int kMoveCtas = 8 * 148;
 
 // Unsigned keys in the order of the scores (-0 = 0, NaN lowest); tokens that
 // always stay are above every score.
@@ -49,39 +54,26 @@ __device__ __forceinline__ Sequence sequence_of(const EvictArgs &p, int b) {
   return q;
 }
 
-// Block id of column `col`, checked against the pool (block 0 otherwise).
+// Block id of column `col`; -1 (and recorded) where it is none of the pool's.
 __device__ __forceinline__ int64_t block_at(const uint32_t *table, int col, int64_t num_blocks) {
-  const uint32_t id = table[col];
+  const uint32_t id = __ldg(table + col);
   if ((int64_t)id < num_blocks) return id;
   raise_device_error(VASR_PA_DERR_BLOCK_RANGE);
   return -1;
 }
 
-// Exclusive prefix sum of x over the block; *total the block's sum.
-__device__ __forceinline__ int block_scan(int x, int *total) {
-  __shared__ int part[kSelectThreads / 32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int s = x;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, s, o);
-    if (lane >= o) s += y;
-  }
-  if (lane == 31) part[warp] = s;
-  __syncthreads();
-  int before = 0, all = 0;
-  for (int w = 0; w < kSelectThreads / 32; ++w) {
-    if (w < warp) before += part[w];
-    all += part[w];
-  }
-  __syncthreads();
-  *total = all;
-  return before + s - x;
-}
-
-// kept[b, h, :] = the indices that stay, ascending, then -1.
-__global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const EvictArgs p) {
-  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+// kept[b, h, :] = the indices that stay, ascending, then -1. key_cap tokens'
+// keys fit the dynamic shared memory; those past them are made anew on every
+// pass.
+__global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const EvictArgs p, int key_cap) {
+  extern __shared__ uint32_t s_key[];
+  __shared__ int hist[256];
+  __shared__ int s_above[kSelectWarps], s_ties[kSelectWarps];
+  __shared__ uint32_t s_prefix;
+  __shared__ int s_rank, s_done;
+  pdl_launch_dependents();
+  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int shift = 31 - __clz(p.block_size);
   const Sequence q = sequence_of(p, b);
   int32_t *kept = p.kept + ((int64_t)b * p.num_kv_heads + h) * p.budget;
   if (h == 0 && tid == 0) p.new_lens[b] = (uint32_t)q.budget;
@@ -90,75 +82,149 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
     for (int i = tid; i < q.budget; i += kSelectThreads) kept[i] = i;
     return;
   }
+  if (q.budget == 0) return;
   const uint32_t *table = p.block_tables + (int64_t)b * p.cols;
-  auto key_of = [&](int j) -> uint32_t {
-    if (j < p.num_sink || j >= q.len - p.num_recent) return 0xffffffffu;
-    const int64_t blk = block_at(table, j / p.block_size, p.num_blocks);
+  const int recent0 = q.len - p.num_recent;
+  auto make_key = [&](int j) -> uint32_t {
+    const int64_t blk = block_at(table, j >> shift, p.num_blocks);
+    if (j < p.num_sink || j >= recent0) return 0xffffffffu;
     if (blk < 0) return 0u;
-    return score_key(p.score_cache[(blk * p.num_kv_heads + h) * p.block_size + j % p.block_size]);
+    return score_key(p.score_cache[((blk * p.num_kv_heads + h) << shift) + (j & (p.block_size - 1))]);
   };
-  // the key of rank `budget` from above: one byte of it per pass
-  __shared__ int hist[256];
-  __shared__ uint32_t s_prefix;
-  __shared__ int s_rank;
+#pragma unroll 4
+  for (int j = tid; j < min(q.len, key_cap); j += kSelectThreads) s_key[j] = make_key(j);
+  auto key_of = [&](int j) { return j < key_cap ? s_key[j] : make_key(j); };
+  // ---- the key of rank `budget` from above, one byte of it per pass
   uint32_t prefix = 0, mask = 0;
   int rank = q.budget;  // 1-based rank among the keys that match the prefix
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    hist[tid] = 0;
+  for (int shift8 = 24; shift8 >= 0; shift8 -= 8) {
+    if (tid < 256) hist[tid] = 0;
     __syncthreads();
-    for (int j = tid; j < q.len; j += kSelectThreads) {
-      const uint32_t key = key_of(j);
-      if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255u], 1);
+    for (int j0 = 0; j0 < q.len; j0 += kSelectThreads) {
+      const int j = j0 + tid;
+      const uint32_t key = j < q.len ? key_of(j) : 0u;
+      const bool in = j < q.len && (key & mask) == prefix;
+      // one count per distinct digit of the warp: scores share their leading bytes
+      const uint32_t digit = in ? (key >> shift8) & 255u : 256u;
+      const uint32_t same = __match_any_sync(0xffffffffu, digit);
+      if (in && lane == __ffs(same) - 1) atomicAdd(&hist[digit], __popc(same));
     }
     __syncthreads();
-    if (tid == 0) {
-      int d = 255;
-      while (d > 0 && rank > hist[d]) rank -= hist[d--];
-      s_prefix = prefix | ((uint32_t)d << shift);
-      s_rank = rank;
+    if (warp == 0) {  // lane l: digits 255 - 8 l downwards; which one holds the rank
+      int c[8], sum = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += c[i] = hist[255 - 8 * lane - i];
+      int upto = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
+      }
+      int before = upto - sum;
+      if (before < rank && rank <= upto) {
+        int i = 0;
+        while (i < 7 && rank > before + c[i]) before += c[i++];
+        s_prefix = prefix | (uint32_t)(255 - 8 * lane - i) << shift8;
+        s_rank = rank - before;
+        s_done = c[i] == rank - before;  // the whole digit stays: the lower bytes do not matter
+      }
     }
     __syncthreads();
     prefix = s_prefix;
     rank = s_rank;
-    mask |= 255u << shift;
-    __syncthreads();
+    mask |= 255u << shift8;
+    if (s_done) break;
   }
-  // above the threshold, or equal to it and among the first `rank` equal ones
-  int done = 0, ties = 0;
-  for (int j0 = 0; j0 < q.len; j0 += kSelectThreads) {
-    const int j = j0 + tid;
-    const uint32_t key = j < q.len ? key_of(j) : 0u;
-    const bool tie = j < q.len && key == prefix;
-    int n;
-    const int tie_at = ties + block_scan(tie, &n);
-    ties += n;
-    const bool keep = j < q.len && (key > prefix || (tie && tie_at < rank));
-    const int at = done + block_scan(keep, &n);
-    done += n;
-    if (keep) kept[at] = j;
+  // ---- kept are the keys above the prefix and the first `rank` equal to it:
+  // each warp counts its stretch of the tokens, then writes it
+  const int per = (q.len + kSelectThreads - 1) / kSelectThreads * 32;  // tokens of a warp
+  const int j0 = warp * per, j1 = min(q.len, j0 + per);
+  int above = 0, ties = 0;
+  for (int j = j0 + lane; j < j1; j += 32) {
+    const uint32_t key = key_of(j);
+    above += key > prefix;
+    ties += key == prefix;
+  }
+  above = __reduce_add_sync(0xffffffffu, above);
+  ties = __reduce_add_sync(0xffffffffu, ties);
+  if (lane == 0) {
+    s_above[warp] = above;
+    s_ties[warp] = ties;
+  }
+  __syncthreads();
+  above = ties = 0;
+  for (int w = 0; w < warp; ++w) {
+    above += s_above[w];
+    ties += s_ties[w];
+  }
+  const uint32_t lower = (1u << lane) - 1u;
+  for (int j = j0; j < j1; j += 32) {
+    const int mine = j + lane;
+    const uint32_t key = mine < j1 ? key_of(mine) : 0u;
+    const bool up = mine < j1 && key > prefix, tie = mine < j1 && key == prefix;
+    const uint32_t ups = __ballot_sync(0xffffffffu, up), eqs = __ballot_sync(0xffffffffu, tie);
+    const int tie_at = ties + __popc(eqs & lower);
+    if (up || (tie && tie_at < rank)) kept[above + __popc(ups & lower) + min(tie_at, rank)] = mine;
+    above += __popc(ups);
+    ties += __popc(eqs);
   }
 }
 
-// One slice of 16 bytes' worth of dims: K, V or the scores of one (sequence,
-// head). Slices [0, nk) are K chunks, [nk, nk + nv) groups of kX V rows, the
-// last one the scores.
+// The move of one (sequence, head), in units that gridDim.x CTAs share: kBatch
+// chunks of K, as many bytes of V rows, or the scores. A thread has a token of
+// the tile, and works out where it comes from and goes to once for all its
+// units. A unit is read before any of it is written; the K chunks and V rows
+// of different units do not touch.
+constexpr int kBatch = 4;
 template <typename U>
-__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictArgs p) {
-  constexpr int kX = 16 / (int)sizeof(U);
-  const int slice = blockIdx.x, h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+constexpr int v_rows() { return 16 / (int)sizeof(U) * kBatch / 2; }
+
+// count (at most N) elements, BS apart, of this thread's token: all threads'
+// reads come before any write when the places overlap.
+template <int N, int BS, typename E>
+__device__ __forceinline__ void move_unit(const E *src, E *dst, int count, bool live, bool in_place) {
+  E v[N];
+  if (live) {
+    if (count == N) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = src[i * BS];
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (i < count) v[i] = src[i * BS];
+    }
+  }
+  if (in_place) __syncthreads();
+  if (live) {
+    if (count == N) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) dst[i * BS] = v[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (i < count) dst[i * BS] = v[i];
+    }
+  }
+}
+
+template <typename U, int BS>
+__global__ void __launch_bounds__(kMoveMostThreads) evict_move_kernel(const EvictArgs p) {
+  constexpr int kX = 16 / (int)sizeof(U), kRows = v_rows<U>();
+  pdl_wait();
+  const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
   const Sequence q = sequence_of(p, b);
-  const uint32_t *out_table = p.out_block_tables ? p.out_block_tables + (int64_t)b * p.out_cols
-                                                 : p.block_tables + (int64_t)b * p.cols;
-  const int out_cols = p.out_block_tables ? p.out_cols : p.cols;
+  const bool in_place = !p.out_block_tables;
+  if (in_place && q.len == q.budget) return;  // everything stays where it is
   const uint32_t *table = p.block_tables + (int64_t)b * p.cols;
+  const uint32_t *out_table = in_place ? table : p.out_block_tables + (int64_t)b * p.out_cols;
   const int32_t *kept = p.kept + ((int64_t)b * p.num_kv_heads + h) * p.budget;
-  const int BS = p.block_size, D = p.head_dim, nk = D / kX;
-  const int budget = min(q.budget, out_cols * BS);
-  for (int r0 = 0; r0 < budget; r0 += kMoveThreads) {
+  const int D = p.head_dim, chunks = D / kX;
+  const int k_units = (chunks + kBatch - 1) / kBatch, units = k_units + (D + kRows - 1) / kRows + 1;
+  for (int r0 = 0; r0 < q.budget; r0 += blockDim.x) {
     const int r = r0 + tid;
-    int64_t from = -1, to = -1;
+    int64_t from = -1, to = -1;  // (block, head)
     int so = 0, dof = 0;
-    if (r < budget) {
+    if (r < q.budget) {
       const int j = kept[r];
       const int64_t sb = block_at(table, j / BS, p.num_blocks), db = block_at(out_table, r / BS, p.num_blocks);
       if (sb >= 0 && db >= 0) {
@@ -168,41 +234,66 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictArg
         dof = r % BS;
       }
     }
-    if (slice < nk) {  // K chunk: 16 bytes a token
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (from >= 0) v = static_cast<const uint4 *>(p.key_cache)[(from * nk + slice) * BS + so];
-      __syncthreads();
-      if (from >= 0) static_cast<uint4 *>(p.key_cache)[(to * nk + slice) * BS + dof] = v;
-    } else if (slice < 2 * nk) {  // kX rows of V
-      U v[kX];
-      const int d0 = (slice - nk) * kX;
-      U *cache = static_cast<U *>(p.value_cache);
-      if (from >= 0)
-        for (int e = 0; e < kX; ++e) v[e] = cache[(from * D + d0 + e) * BS + so];
-      __syncthreads();
-      if (from >= 0)
-        for (int e = 0; e < kX; ++e) cache[(to * D + d0 + e) * BS + dof] = v[e];
-    } else {
-      float s = 0.f;
-      if (from >= 0) s = p.score_cache[from * BS + so];
-      __syncthreads();
-      if (from >= 0) p.score_cache[to * BS + dof] = s;
+    const bool live = from >= 0;
+    for (int u = blockIdx.x; u < units; u += gridDim.x) {
+      if (u < k_units) {  // K: 16 bytes a token and chunk
+        const int c0 = u * kBatch;
+        uint4 *cache = static_cast<uint4 *>(p.key_cache);
+        move_unit<kBatch, BS>(cache + (from * chunks + c0) * BS + so, cache + (to * chunks + c0) * BS + dof,
+                              min(kBatch, chunks - c0), live, in_place);
+      } else if (u < units - 1) {  // V: an element a token and row, the tile's tokens along the rows
+        const int d0 = (u - k_units) * kRows;
+        U *cache = static_cast<U *>(p.value_cache);
+        move_unit<kRows, BS>(cache + (from * D + d0) * BS + so, cache + (to * D + d0) * BS + dof, min(kRows, D - d0),
+                             live, in_place);
+      } else {
+        move_unit<1, BS>(p.score_cache + from * BS + so, p.score_cache + to * BS + dof, 1, live, in_place);
+      }
     }
   }
 }
 
+// CTAs per (sequence, head): enough to fill the SMs, at most one per unit.
+// Where even that leaves SMs idle, tiles of 1024 tokens take fewer turns.
+template <typename U, int BS>
+int launch_move_bs(const EvictArgs &a, cudaStream_t s) {
+  const int chunks = a.head_dim * (int)sizeof(U) / 16;
+  const int64_t pairs = (int64_t)a.num_seqs * a.num_kv_heads;
+  const int units = (chunks + kBatch - 1) / kBatch + (a.head_dim + v_rows<U>() - 1) / v_rows<U>() + 1;
+  int64_t parts = (kMoveCtas + pairs - 1) / pairs;
+  parts = parts > units ? units : parts;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)parts, (unsigned)a.num_kv_heads, (unsigned)a.num_seqs);
+  cfg.blockDim = dim3(pairs * parts < kMoveCtas / 4 && a.budget > kMoveThreads ? kMoveMostThreads : kMoveThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, evict_move_kernel<U, BS>, a) == cudaSuccess ? VASR_PA_OK : VASR_PA_ELAUNCH;
+}
+
 template <typename U>
 int launch_move(const EvictArgs &a, cudaStream_t s) {
-  const dim3 grid((unsigned)(2 * (a.head_dim * (int)sizeof(U) / 16) + 1), (unsigned)a.num_kv_heads,
-                  (unsigned)a.num_seqs);
-  evict_move_kernel<U><<<grid, kMoveThreads, 0, s>>>(a);
-  return cudaPeekAtLastError() == cudaSuccess ? VASR_PA_OK : VASR_PA_ELAUNCH;
+  switch (a.block_size) {
+    case 8: return launch_move_bs<U, 8>(a, s);
+    case 16: return launch_move_bs<U, 16>(a, s);
+    default: return launch_move_bs<U, 32>(a, s);
+  }
 }
 
 }  // namespace
 
 int launch_evict(const EvictArgs &a, cudaStream_t s) {
-  evict_select_kernel<<<dim3((unsigned)a.num_kv_heads, (unsigned)a.num_seqs), kSelectThreads, 0, s>>>(a);
+  // keys in shared memory: 32 KB a CTA, or most of an SM's where there are few CTAs
+  constexpr int kMostKeys = 49152;
+  const int64_t pairs = (int64_t)a.num_seqs * a.num_kv_heads;
+  int key_cap = a.max_context_len < 8192 || pairs > 148 ? 8192 : kMostKeys;
+  if (key_cap > a.max_context_len) key_cap = a.max_context_len;
+  static std::atomic<uint64_t> attr_done{0};
+  if (!ensure_smem_attr(evict_select_kernel, kMostKeys * 4, attr_done)) return VASR_PA_ELAUNCH;
+  evict_select_kernel<<<dim3((unsigned)a.num_kv_heads, (unsigned)a.num_seqs), kSelectThreads, key_cap * 4, s>>>(a, key_cap);
   switch (a.elem_size) {
     case 1: return launch_move<uint8_t>(a, s);
     case 2: return launch_move<uint16_t>(a, s);
