@@ -52,10 +52,15 @@ struct MmaLayout {
 MmaLayout mma_layout(int num_seqs, int query_len, int score_rows, int num_heads, int num_kv_heads, int block_size,
                      int max_context_len) {
   MmaLayout l;
-  // halve the splits until the grid has two CTAs per SM
-  int tokens = kMmaSplitTokens;
-  while (tokens > 64 && (int64_t)num_seqs * num_kv_heads * ((max_context_len + tokens - 1) / tokens) < 2 * 148) tokens >>= 1;
-  l.pages_per_split = tokens / block_size < 1 ? 1 : tokens / block_size;
+  // Splits of 1024 tokens, or shorter ones that just fill the SMs once (three
+  // CTAs each) where the longest contexts would leave some idle; at least 64.
+  const int64_t pairs = (int64_t)num_seqs * num_kv_heads;
+  const int pages = (max_context_len + block_size - 1) / block_size;
+  int64_t per_pair = 3 * 148 / pairs;
+  if (per_pair < 1) per_pair = 1;
+  int64_t want = (pages + per_pair - 1) / per_pair;
+  const int least = (64 + block_size - 1) / block_size, most = kMmaSplitTokens / block_size;
+  l.pages_per_split = (int)(want < least ? least : want > most ? most : want);
   if (l.pages_per_split > kScoredMaxPages) l.pages_per_split = kScoredMaxPages;
   const int per = l.pages_per_split * block_size;
   l.max_splits = (max_context_len + per - 1) / per;
@@ -299,10 +304,17 @@ int launch_mma_rows(const ScoredArgs &a, cudaStream_t s) {
   const dim3 grid((unsigned)l.max_splits, (unsigned)(a.num_kv_heads * p.row_tiles), (unsigned)a.num_seqs);
   kern<<<grid, kScoredThreads, C::kSmemBytes, s>>>(p);
   if (!p.fused) {
-    const int merge = (p.rows + 3) / 4;
     const int chunks = (a.max_context_len + kJoinTokens - 1) / kJoinTokens;
-    scored_join_kernel<T><<<dim3((unsigned)(merge + chunks), (unsigned)a.num_kv_heads, (unsigned)a.num_seqs),
-                            kScoredThreads, 0, s>>>(p, BS, merge);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(p.rows + chunks), (unsigned)a.num_kv_heads, (unsigned)a.num_seqs);
+    cfg.blockDim = dim3(kScoredThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, scored_join_kernel<T>, p, BS) == cudaSuccess ? VASR_PA_OK : VASR_PA_ELAUNCH;
   }
   return cudaPeekAtLastError() == cudaSuccess ? VASR_PA_OK : VASR_PA_ELAUNCH;
 }

@@ -72,6 +72,14 @@ struct ScoredMmaParams {
   float decay;
 };
 
+// 2^x in one instruction (2 ulp, results below 2^-126 are 0): the arguments
+// are a score less its row's maximum, whose own rounding is larger.
+__device__ __forceinline__ float scored_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // The context length a kernel works with; too long a one is cut and recorded.
 __device__ __forceinline__ int scored_context(const ScoredMmaParams &p, int b, int bs, bool report) {
   int64_t n = p.context_lens[b];
@@ -88,51 +96,56 @@ __device__ __forceinline__ int scored_splits(int n, int pages_per_split, int bs)
   return (n + per - 1) / per;
 }
 
-// (m, 1 / l) of rows [0, count) over the splits, into shared memory. A row
-// that saw nothing gets (0, 0): its raw scores are -inf and weigh 0.
-__device__ __forceinline__ void scored_final_rows(const ScoredMmaParams &p, int64_t pair, int n_splits, int count,
-                                                  float2 *fin) {
-  for (int r = threadIdx.x; r < count; r += kScoredThreads) {
-    const float2 *ml = p.ws_ml + pair * p.max_splits * p.rows + r;
-    float m = -INFINITY, l = 0.f;
-    for (int s = 0; s < n_splits; ++s) m = fmaxf(m, __ldcg(&ml[(int64_t)s * p.rows].x));
-    for (int s = 0; s < n_splits; ++s) {
-      const float2 v = __ldcg(&ml[(int64_t)s * p.rows]);
-      if (v.y != 0.f) l = fmaf(v.y, exp2f(v.x - m), l);
-    }
-    fin[r] = l != 0.f ? make_float2(m, 1.f / l) : make_float2(0.f, 0.f);
+// (m, 1 / l) of one row over the splits, by one warp. A row that saw nothing
+// gets (0, 0): its raw scores are -inf and weigh 0.
+__device__ __forceinline__ float2 scored_final_row(const ScoredMmaParams &p, int64_t pair, int n_splits, int r) {
+  const int lane = threadIdx.x & 31;
+  const float2 *ml = p.ws_ml + pair * p.max_splits * p.rows + r;
+  float m = -INFINITY, l = 0.f;
+  for (int s = lane; s < n_splits; s += 32) {
+    const float2 v = __ldcg(&ml[(int64_t)s * p.rows]);
+    const float m_new = fmaxf(m, v.x);
+    if (v.y != 0.f) l = (l != 0.f ? l * scored_exp2(m - m_new) : 0.f) + v.y * scored_exp2(v.x - m_new);
+    m = m_new;
   }
+  const float top = warp_max_xor(m, 32);
+  l = warp_sum_xor(l != 0.f ? l * scored_exp2(m - top) : 0.f, 32);
+  return l != 0.f ? make_float2(top, 1.f / l) : make_float2(0.f, 0.f);
 }
 
-// Rows [r0, r1) of the output from the splits' partials.
-template <typename T>
-__device__ __forceinline__ void scored_merge_rows(const ScoredMmaParams &p, int b, int kvh, int n_splits, int r0, int r1,
-                                                  const float2 *fin, float v_mul) {
-  constexpr int D = kScoredDim;
-  const int64_t slot0 = ((int64_t)b * p.num_kv_heads + kvh) * p.max_splits;
-  for (int e = threadIdx.x; e < (r1 - r0) * (D / 4); e += kScoredThreads) {
-    const int r = r0 + e / (D / 4), d = e % (D / 4) * 4;
-    const float2 f = fin[r];
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < n_splits; ++s) {
-      const int64_t at = (slot0 + s) * p.rows + r;
-      const float2 ml = __ldcg(&p.ws_ml[at]);
-      if (ml.y == 0.f) continue;
-      const float w = exp2f(ml.x - f.x);
-      const float4 v = __ldcg(reinterpret_cast<const float4 *>(p.ws_o + at * D + d));
+// 4 dims of a row from its partials of splits first, first + step, ..., by one
+// warp (lane: dims 4 lane ..).
+__device__ __forceinline__ float4 scored_sum_splits(const ScoredMmaParams &p, int64_t pair, int n_splits, int r, float m,
+                                                    int first, int step) {
+  const int lane = threadIdx.x & 31;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int s = first; s < n_splits; s += step) {
+    const int64_t at = (pair * p.max_splits + s) * p.rows + r;
+    const float2 ml = __ldcg(&p.ws_ml[at]);
+    const float4 v = __ldcg(reinterpret_cast<const float4 *>(p.ws_o + at * kScoredDim) + lane);
+    const float w = ml.y != 0.f ? scored_exp2(ml.x - m) : 0.f;
+    if (w != 0.f) {  // a partial of weight 0 may hold anything
       o.x = fmaf(v.x, w, o.x);
       o.y = fmaf(v.y, w, o.y);
       o.z = fmaf(v.z, w, o.z);
       o.w = fmaf(v.w, w, o.w);
     }
-    const float mul = f.y * v_mul;
-    T *out = static_cast<T *>(p.out) +
-             (((int64_t)b * p.query_len + r / p.group) * p.num_heads + kvh * p.group + r % p.group) * D + d;
-    out[0] = Elem<T>::from_f32(o.x * mul);
-    out[1] = Elem<T>::from_f32(o.y * mul);
-    out[2] = Elem<T>::from_f32(o.z * mul);
-    out[3] = Elem<T>::from_f32(o.w * mul);
   }
+  return o;
+}
+
+template <typename T>
+__device__ __forceinline__ T *scored_out_row(const ScoredMmaParams &p, int b, int kvh, int r) {
+  return static_cast<T *>(p.out) +
+         (((int64_t)b * p.query_len + r / p.group) * p.num_heads + kvh * p.group + r % p.group) * kScoredDim;
+}
+template <typename T>
+__device__ __forceinline__ void scored_store4(T *out, float4 o, float mul) {
+  out[0] = Elem<T>::from_f32(o.x * mul);
+  out[1] = Elem<T>::from_f32(o.y * mul);
+  out[2] = Elem<T>::from_f32(o.z * mul);
+  out[3] = Elem<T>::from_f32(o.w * mul);
 }
 
 // score <- decay score + sum of the scored rows' weights, tokens [j0, j1), 4
@@ -150,10 +163,10 @@ __device__ __forceinline__ void scored_add_weights(const ScoredMmaParams &p, int
     for (int r = 0; r < p.scored_rows; ++r) {
       const float2 f = fin[r];
       const float4 v = __ldcg(reinterpret_cast<const float4 *>(x + r * p.x_stride + j));
-      w.x = fmaf(exp2f(v.x - f.x), f.y, w.x);
-      w.y = fmaf(exp2f(v.y - f.x), f.y, w.y);
-      w.z = fmaf(exp2f(v.z - f.x), f.y, w.z);
-      w.w = fmaf(exp2f(v.w - f.x), f.y, w.w);
+      w.x = fmaf(scored_exp2(v.x - f.x), f.y, w.x);
+      w.y = fmaf(scored_exp2(v.y - f.x), f.y, w.y);
+      w.z = fmaf(scored_exp2(v.z - f.x), f.y, w.z);
+      w.w = fmaf(scored_exp2(v.w - f.x), f.y, w.w);
     }
     const int left = j1 - j;  // places past the context keep their bits
     float4 s = old;
@@ -322,6 +335,7 @@ __global__ void __launch_bounds__(kScoredThreads, MINB) scored_mma_kernel(const 
     const uint32_t sv = s_base + C::kOffV + s * C::kSP * C::kPB;
     const int unit0 = u * C::kST;              // first token, relative to tok0
     const int valid = tok1 - tok0 - unit0;     // cached tokens of the stage
+    const int whole = min(valid, n_all - tok0 - unit0);  // those that every row sees
 #pragma unroll
     for (int ti = 0; ti < C::kTiles; ++ti) {
       const int t0 = ti * 16;
@@ -355,8 +369,10 @@ __global__ void __launch_bounds__(kScoredThreads, MINB) scored_mma_kernel(const 
           dec_mma<TM>(sacc[1], qa[ks][0], a1, qa[ks][1], a3, b2, b3);
         }
       }
-      // ---- raw scores of the lane's rows, tokens tok(n, e) of the tile
+      // ---- raw scores of the lane's rows, tokens tok(n, e) of the tile; only
+      // a tile that not all rows see all of needs masks
       auto tok = [&](int nn, int e) { return kFp8 ? t0 + 4 * tig + 2 * nn + e : t0 + nn * 8 + tig * 2 + e; };
+      const bool tail = t0 + 16 > whole;
       float pv[NRT][4];
       uint32_t pa[NRT][2];
 #pragma unroll
@@ -364,21 +380,27 @@ __global__ void __launch_bounds__(kScoredThreads, MINB) scored_mma_kernel(const 
         float x[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float v = sacc[e >> 1][2 * t + (e & 1)] * c_log2[t];
-          if (use_softcap) v = p.softcap * tanhf(v / p.softcap) * kLog2e;
-          const int j = tok(e >> 1, e & 1);
-          x[e] = j < valid && unit0 + j < seen[t] ? v : -INFINITY;
+          x[e] = sacc[e >> 1][2 * t + (e & 1)] * c_log2[t];
+          if (use_softcap) x[e] = p.softcap * tanhf(x[e] / p.softcap) * kLog2e;
+        }
+        if (tail) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int j = tok(e >> 1, e & 1);
+            if (j >= valid || unit0 + j >= seen[t]) x[e] = -INFINITY;
+          }
         }
         if (xrow[t]) {
-          if (tok(0, 0) < valid) *reinterpret_cast<float2 *>(xrow[t] + unit0 + tok(0, 0)) = make_float2(x[0], x[1]);
-          if (tok(1, 0) < valid) *reinterpret_cast<float2 *>(xrow[t] + unit0 + tok(1, 0)) = make_float2(x[2], x[3]);
+          float *at = xrow[t] + unit0;
+          if (tok(0, 0) < valid) *reinterpret_cast<float2 *>(at + tok(0, 0)) = make_float2(x[0], x[1]);
+          if (tok(1, 0) < valid) *reinterpret_cast<float2 *>(at + tok(1, 0)) = make_float2(x[2], x[3]);
         }
         float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
         if (__any_sync(0xffffffffu, mx > m_used[t] + kRescale)) {
           const float m_new = fmaxf(m_used[t], mx);
-          const float alpha = m_used[t] == -INFINITY ? 0.f : exp2f(m_used[t] - m_new);
+          const float alpha = m_used[t] == -INFINITY ? 0.f : scored_exp2(m_used[t] - m_new);
           m_used[t] = m_new;
           l_part[t] *= alpha;
           // O^T's columns 2 tig, 2 tig + 1 are rows whose alphas live in lanes 8 tig, 8 tig + 4
@@ -391,9 +413,10 @@ __global__ void __launch_bounds__(kScoredThreads, MINB) scored_mma_kernel(const 
             o[t][j][3] *= a1;
           }
         }
+        const float off = m_used[t] == -INFINITY ? 0.f : m_used[t];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          pv[t][e] = x[e] == -INFINITY ? 0.f : exp2f(x[e] - (m_used[t] == -INFINITY ? 0.f : m_used[t]));
+          pv[t][e] = scored_exp2(x[e] - off);
           l_part[t] += pv[t][e];
         }
 #pragma unroll
@@ -408,8 +431,6 @@ __global__ void __launch_bounds__(kScoredThreads, MINB) scored_mma_kernel(const 
         }
       }
       // ---- O^T += V^T P^T over the tokens that every row sees
-      const int whole = min(valid, n_all - tok0 - unit0);  // tokens of the stage below n_all
-      const bool tail = t0 + 16 > whole;
       if constexpr (kFp8) {
         const int vd = (lane >> 3) * 8 + (lane & 7);
         const uint32_t vrow = sv + (t0 / BS) * C::kPB + vd * BS + t0 % BS;
@@ -535,7 +556,7 @@ __global__ void __launch_bounds__(kScoredThreads, MINB) scored_mma_kernel(const 
     for (int w = 0; w < C::kWarps; ++w) {
       const float2 ml = cml[w * 16 + r];
       if (ml.y == 0.f) continue;
-      const float f = exp2f(ml.x - m);
+      const float f = scored_exp2(ml.x - m);
       l = fmaf(ml.y, f, l);
       ov = fmaf(co[(w * kRows + r) * D + d], f, ov);
     }
@@ -564,38 +585,58 @@ __global__ void __launch_bounds__(kScoredThreads, MINB) scored_mma_kernel(const 
     __syncthreads();
     if (!flag[0]) return;
     if (tid == 0) p.counters[pair] = 0u;
-    scored_final_rows(p, pair, n_splits, p.rows, fin);
-    __syncthreads();
-    scored_merge_rows<T>(p, b, kvh, n_splits, 0, p.rows, fin, v_mul);
-  } else {
-    __syncthreads();  // fin, and this CTA's raw scores
+    for (int r = warp; r < p.rows; r += C::kWarps) {
+      const float2 f = scored_final_row(p, pair, n_splits, r);
+      const float4 ov = scored_sum_splits(p, pair, n_splits, r, f.x, 0, 1);
+      scored_store4(scored_out_row<T>(p, b, kvh, r) + 4 * lane, ov, f.y * v_mul);
+      if (lane == 0) fin[r] = f;
+    }
   }
+  __syncthreads();  // fin, and in the case of one split this CTA's raw scores
   scored_add_weights(p, b, kvh, BS, 0, n, fin);
 }
 
 // The end of every (sequence, kv head) as a launch of its own, for long
-// contexts: blocks [0, merge_blocks) join 4 rows each, the others add the
-// weights of kJoinTokens tokens each.
+// contexts: blocks [0, rows) join a row each, the others add the weights of
+// kJoinTokens tokens each.
 constexpr int kJoinTokens = 1024;
 template <typename T>
-__global__ void __launch_bounds__(kScoredThreads) scored_join_kernel(const ScoredMmaParams p, int bs, int merge_blocks) {
+__global__ void __launch_bounds__(kScoredThreads) scored_join_kernel(const ScoredMmaParams p, int bs) {
   __shared__ float2 fin[kScoredMaxRows];
+  __shared__ float4 part[kScoredThreads];
   pdl_wait();
-  const int kvh = blockIdx.y, b = blockIdx.z;
+  const int kvh = blockIdx.y, b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kWarps = kScoredThreads / 32;
   const int n = scored_context(p, b, bs, false);
   const int n_splits = scored_splits(n, p.pages_per_split, bs);
   const int64_t pair = (int64_t)b * p.num_kv_heads + kvh;
-  const bool merge = (int)blockIdx.x < merge_blocks;
-  const int j0 = ((int)blockIdx.x - merge_blocks) * kJoinTokens;
-  if (n == 0 || (!merge && j0 >= n)) return;
-  scored_final_rows(p, pair, n_splits, merge ? p.rows : p.scored_rows, fin);
-  __syncthreads();
-  if (merge) {
-    const int r0 = blockIdx.x * 4;
-    scored_merge_rows<T>(p, b, kvh, n_splits, r0, min(r0 + 4, p.rows), fin, p.v_scale ? __ldg(p.v_scale) : 1.f);
-  } else {
-    scored_add_weights(p, b, kvh, bs, j0, min(n, j0 + kJoinTokens), fin);
+  if (n == 0) return;
+  if ((int)blockIdx.x < p.rows) {  // the warps share the splits
+    const int r = blockIdx.x;
+    const float2 f = scored_final_row(p, pair, n_splits, r);
+    part[threadIdx.x] = scored_sum_splits(p, pair, n_splits, r, f.x, warp, kWarps);
+    __syncthreads();
+    if (warp != 0) return;
+    float4 o = part[lane];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) {
+      const float4 v = part[w * 32 + lane];
+      o.x += v.x;
+      o.y += v.y;
+      o.z += v.z;
+      o.w += v.w;
+    }
+    scored_store4(scored_out_row<T>(p, b, kvh, r) + 4 * lane, o, f.y * (p.v_scale ? __ldg(p.v_scale) : 1.f));
+    return;
   }
+  const int j0 = ((int)blockIdx.x - p.rows) * kJoinTokens;
+  if (j0 >= n) return;
+  for (int r = warp; r < p.scored_rows; r += kWarps) {
+    const float2 f = scored_final_row(p, pair, n_splits, r);
+    if (lane == 0) fin[r] = f;
+  }
+  __syncthreads();
+  scored_add_weights(p, b, kvh, bs, j0, min(n, j0 + kJoinTokens), fin);
 }
 
 }  // namespace vasr
