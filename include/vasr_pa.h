@@ -508,9 +508,8 @@ int32_t vasr_pa_fused_qk_norm_mrope_append(
  * added in a fixed order. Block tables of different sequences must not name
  * the same block (it would be scored by both at once), except for the null
  * block that padding rows share, whose scores mean nothing. f32, bf16 or f16
- * queries over pages of the same type or fp8. workspace: zeroed once before
- * first use and left zeroed where it has to be, so calls of any shape may
- * share it; one call at a time per workspace.
+ * queries over pages of the same type or fp8; the workspace is scratch that
+ * needs no clearing, one call at a time.
  */
 size_t vasr_pa_paged_attention_scored_workspace_size(int32_t num_seqs, int32_t query_len,
                                                      int32_t score_rows, int32_t num_heads,

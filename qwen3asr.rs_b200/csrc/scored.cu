@@ -28,11 +28,6 @@ constexpr int kWeightThreads = 256;
 
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
-// Arrival counters of the tensor-core kernel: a fixed region that every call
-// leaves at zero, so that one zeroed workspace serves calls of any shape.
-constexpr int64_t kMaxCounters = 65536;
-constexpr size_t kCounterBytes = kMaxCounters * sizeof(uint32_t);
-
 // ---- tensor-core kernel: which calls it takes, its splits and its workspace
 bool takes_mma(const ScoredArgs &a) {
   return a.dtype != VASR_PA_F32 && a.head_dim == kScoredDim &&
@@ -42,12 +37,11 @@ bool takes_mma(const ScoredArgs &a) {
 }
 
 constexpr int kMmaSplitTokens = 1024;
-constexpr int kMmaFusedContext = 4096;
 
 struct MmaLayout {
   int pages_per_split, max_splits;
   int64_t x_stride;
-  size_t off_counters, off_o, off_ml, off_x, total;
+  size_t off_o, off_ml, off_x, total;
 };
 MmaLayout mma_layout(int num_seqs, int query_len, int score_rows, int num_heads, int num_kv_heads, int block_size,
                      int max_context_len) {
@@ -66,8 +60,7 @@ MmaLayout mma_layout(int num_seqs, int query_len, int score_rows, int num_heads,
   l.max_splits = (max_context_len + per - 1) / per;
   l.x_stride = (int64_t)l.max_splits * per;
   const size_t rows = (size_t)num_seqs * num_kv_heads * l.max_splits * query_len * (num_heads / num_kv_heads);
-  l.off_counters = 0;
-  l.off_o = kCounterBytes;
+  l.off_o = 0;
   l.off_ml = align256(l.off_o + rows * kScoredDim * sizeof(float));
   l.off_x = align256(l.off_ml + rows * sizeof(float2));
   l.total = l.off_x + align256((size_t)num_seqs * score_rows * num_heads * l.x_stride * sizeof(float));
@@ -85,7 +78,7 @@ ScoredLayout layout(int num_seqs, int query_len, int score_rows, int num_heads, 
   l.splits = (max_context_len + kSplitTokens - 1) / kSplitTokens;
   l.x_stride = (int64_t)l.splits * kSplitTokens;
   const size_t rows = (size_t)num_seqs * query_len * num_heads;
-  l.off_o = kCounterBytes;
+  l.off_o = 0;
   l.off_ml = align256(l.off_o + rows * l.splits * head_dim * sizeof(float));
   l.off_x = align256(l.off_ml + rows * (l.splits + 1) * sizeof(float2));
   l.total = l.off_x + align256((size_t)num_seqs * score_rows * num_heads * l.x_stride * sizeof(float));
@@ -279,7 +272,6 @@ int launch_mma_rows(const ScoredArgs &a, cudaStream_t s) {
   p.ws_o = reinterpret_cast<float *>(ws + l.off_o);
   p.ws_ml = reinterpret_cast<float2 *>(ws + l.off_ml);
   p.ws_x = reinterpret_cast<float *>(ws + l.off_x);
-  p.counters = reinterpret_cast<uint32_t *>(ws + l.off_counters);
   p.q_token_stride = a.q_token_stride;
   p.num_blocks = a.num_blocks;
   p.x_stride = l.x_stride;
@@ -294,7 +286,8 @@ int launch_mma_rows(const ScoredArgs &a, cudaStream_t s) {
   p.max_context = a.max_context_len;
   p.pages_per_split = l.pages_per_split;
   p.max_splits = l.max_splits;
-  p.fused = a.max_context_len <= kMmaFusedContext && (int64_t)a.num_seqs * a.num_kv_heads <= kMaxCounters;
+  const int split_tokens = l.pages_per_split * BS;
+  p.x_tokens = (size_t)p.scored_rows * split_tokens * sizeof(float) <= (size_t)C::kXBytes ? split_tokens : 0;
   p.scale = a.scale;
   p.softcap = a.softcapping;
   p.decay = a.decay;
@@ -303,26 +296,32 @@ int launch_mma_rows(const ScoredArgs &a, cudaStream_t s) {
   if (!ensure_smem_attr(kern, C::kSmemBytes, attr_done)) return VASR_PA_ELAUNCH;
   const dim3 grid((unsigned)l.max_splits, (unsigned)(a.num_kv_heads * p.row_tiles), (unsigned)a.num_seqs);
   kern<<<grid, kScoredThreads, C::kSmemBytes, s>>>(p);
-  if (!p.fused) {
-    const int chunks = (a.max_context_len + kJoinTokens - 1) / kJoinTokens;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(p.rows + chunks), (unsigned)a.num_kv_heads, (unsigned)a.num_seqs);
-    cfg.blockDim = dim3(kScoredThreads);
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, scored_join_kernel<T>, p, BS) == cudaSuccess ? VASR_PA_OK : VASR_PA_ELAUNCH;
-  }
-  return cudaPeekAtLastError() == cudaSuccess ? VASR_PA_OK : VASR_PA_ELAUNCH;
+  if (l.max_splits == 1 && p.row_tiles == 1) return cudaPeekAtLastError() == cudaSuccess ? VASR_PA_OK : VASR_PA_ELAUNCH;
+  // the join: as many tokens a CTA as leave about 16 CTAs per SM, 512 at least
+  const int64_t pairs = (int64_t)a.num_seqs * a.num_kv_heads;
+  int chunk = 512;
+  while (chunk < a.max_context_len && pairs * ((a.max_context_len + chunk - 1) / chunk) > 16 * 148) chunk *= 2;
+  const int chunks = (a.max_context_len + chunk - 1) / chunk;
+  const int row_warps = l.max_splits <= 8 ? 1 : kScoredThreads / 32;
+  const int row_ctas = (p.rows * row_warps + kScoredThreads / 32 - 1) / (kScoredThreads / 32);
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = dim3((unsigned)(chunks + row_ctas), (unsigned)a.num_kv_heads, (unsigned)a.num_seqs);
+  cfg.blockDim = dim3(kScoredThreads);
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  return cudaLaunchKernelEx(&cfg, scored_join_kernel<T>, p, BS, chunk, chunks, row_warps) == cudaSuccess ? VASR_PA_OK : VASR_PA_ELAUNCH;
 }
 
 template <typename T, typename TC, int BS>
 int launch_mma_bs(const ScoredArgs &a, cudaStream_t s) {
   const int rows = a.query_len * (a.num_heads / a.num_kv_heads);
-  if (rows <= 4) return launch_mma_rows<T, TC, BS, 1, true>(a, s);
+  // bf16 over fp8 pages: P is rounded to f16, 8 times finer than the output; doubled rows would gain nothing
+  constexpr bool kDup = !(std::is_same<T, __nv_bfloat16>::value && sizeof(TC) == 1);
+  if (rows <= 4 && kDup) return launch_mma_rows<T, TC, BS, 1, kDup>(a, s);
   if (rows <= 8) return launch_mma_rows<T, TC, BS, 1, false>(a, s);
   return launch_mma_rows<T, TC, BS, 2, false>(a, s);
 }
