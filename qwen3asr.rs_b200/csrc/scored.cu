@@ -12,10 +12,12 @@
 // context does not have: each split leaves its raw scores x (log2 domain) and
 // its partial (o, m, l) in the workspace, a merge makes out and the final
 // (m, l) of every row, and the last step turns the raw scores into weights.
-// 16-bit queries at head_dim 128 run scored_mma_kernel (scored_mma.cuh); the
-// kernels here serve f32 and the other shapes.
+// head_dim 128 runs scored_mma_kernel (16-bit queries, scored_mma.cuh) or
+// scored_f32_kernel (f32 queries and pages, scored_f32.cuh); the kernels here
+// serve the other shapes, one thread a token, three launches.
 #include "common.cuh"
 #include "launch.h"
+#include "scored_f32.cuh"
 #include "scored_mma.cuh"
 
 namespace vasr {
@@ -28,24 +30,24 @@ constexpr int kWeightThreads = 256;
 
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
-// ---- tensor-core kernel: which calls it takes, its splits and its workspace
-bool takes_mma(const ScoredArgs &a) {
-  return a.dtype != VASR_PA_F32 && a.head_dim == kScoredDim &&
-         a.query_len * (a.num_heads / a.num_kv_heads) <= kScoredMaxRows &&
-         !(a.cache_dtype == VASR_PA_FP8_E4M3 && a.block_size < 16) &&
-         (int64_t)a.num_kv_heads * ((a.query_len * (a.num_heads / a.num_kv_heads) + 7) / 8) <= 65535;
+// ---- the split kernels: which calls they take, their splits and workspace
+bool takes_split(const ScoredArgs &a) {
+  const int rows = a.query_len * (a.num_heads / a.num_kv_heads);
+  const bool fp8 = a.cache_dtype == VASR_PA_FP8_E4M3;
+  return a.head_dim == kScoredDim && rows <= kScoredMaxRows && !(fp8 && (a.block_size < 16 || a.dtype == VASR_PA_F32)) &&
+         (int64_t)a.num_kv_heads * ((rows + 1) / 2) <= 65535;
 }
 
-constexpr int kMmaSplitTokens = 1024;
+constexpr int kSplitMostTokens = 1024;
 
-struct MmaLayout {
+struct SplitLayout {
   int pages_per_split, max_splits;
   int64_t x_stride;
   size_t off_o, off_ml, off_x, total;
 };
-MmaLayout mma_layout(int num_seqs, int query_len, int score_rows, int num_heads, int num_kv_heads, int block_size,
+SplitLayout split_layout(int num_seqs, int query_len, int score_rows, int num_heads, int num_kv_heads, int block_size,
                      int max_context_len) {
-  MmaLayout l;
+  SplitLayout l;
   // Splits of 1024 tokens, or shorter ones that just fill the SMs once (three
   // CTAs each) where the longest contexts would leave some idle; at least 64.
   const int64_t pairs = (int64_t)num_seqs * num_kv_heads;
@@ -53,7 +55,7 @@ MmaLayout mma_layout(int num_seqs, int query_len, int score_rows, int num_heads,
   int64_t per_pair = 3 * 148 / pairs;
   if (per_pair < 1) per_pair = 1;
   int64_t want = (pages + per_pair - 1) / per_pair;
-  const int least = (64 + block_size - 1) / block_size, most = kMmaSplitTokens / block_size;
+  const int least = (64 + block_size - 1) / block_size, most = kSplitMostTokens / block_size;
   l.pages_per_split = (int)(want < least ? least : want > most ? most : want);
   if (l.pages_per_split > kScoredMaxPages) l.pages_per_split = kScoredMaxPages;
   const int per = l.pages_per_split * block_size;
@@ -250,16 +252,14 @@ int launch_scored_t(const ScoredArgs &a, cudaStream_t s) {
   return cudaPeekAtLastError() == cudaSuccess ? VASR_PA_OK : VASR_PA_ELAUNCH;
 }
 
-template <typename T, typename TC, int BS, int NRT, bool kDup>
-int launch_mma_rows(const ScoredArgs &a, cudaStream_t s) {
-  constexpr int kStage = 2 * (BS < 16 ? 16 : BS) * kScoredDim * (int)sizeof(TC);
-  constexpr int kNST = kStage <= 4096 ? 8 : kStage <= 8192 ? 8 : 4;
-  constexpr int kMinB = sizeof(TC) == 1 && NRT == 1 ? 4 : 3;
-  using C = ScoredCfg<TC, BS, kNST>;
-  const MmaLayout l = mma_layout(a.num_seqs, a.query_len, a.score_rows, a.num_heads, a.num_kv_heads, a.block_size,
+// Launches kern, a split kernel of tiles of tile_rows rows, and the join where one is needed.
+template <typename T, typename C, int BS>
+int launch_split(const ScoredArgs &a, void (*kern)(ScoredSplitParams), std::atomic<uint64_t> &attr_done, int tile_rows,
+                 cudaStream_t s) {
+  const SplitLayout l = split_layout(a.num_seqs, a.query_len, a.score_rows, a.num_heads, a.num_kv_heads, a.block_size,
                                  a.max_context_len);
   unsigned char *ws = static_cast<unsigned char *>(a.workspace);
-  ScoredMmaParams p{};
+  ScoredSplitParams p{};
   p.out = a.out;
   p.q = a.query;
   p.k_cache = a.key_cache;
@@ -281,7 +281,7 @@ int launch_mma_rows(const ScoredArgs &a, cudaStream_t s) {
   p.query_len = a.query_len;
   p.rows = a.query_len * p.group;
   p.scored_rows = a.score_rows * p.group;
-  p.row_tiles = kDup ? 1 : (p.rows + 8 * NRT - 1) / (8 * NRT);
+  p.row_tiles = (p.rows + tile_rows - 1) / tile_rows;
   p.cols = a.max_num_blocks_per_seq;
   p.max_context = a.max_context_len;
   p.pages_per_split = l.pages_per_split;
@@ -291,8 +291,6 @@ int launch_mma_rows(const ScoredArgs &a, cudaStream_t s) {
   p.scale = a.scale;
   p.softcap = a.softcapping;
   p.decay = a.decay;
-  auto kern = scored_mma_kernel<T, TC, BS, NRT, kDup, kNST, kMinB>;
-  static std::atomic<uint64_t> attr_done{0};
   if (!ensure_smem_attr(kern, C::kSmemBytes, attr_done)) return VASR_PA_ELAUNCH;
   const dim3 grid((unsigned)l.max_splits, (unsigned)(a.num_kv_heads * p.row_tiles), (unsigned)a.num_seqs);
   kern<<<grid, kScoredThreads, C::kSmemBytes, s>>>(p);
@@ -316,6 +314,35 @@ int launch_mma_rows(const ScoredArgs &a, cudaStream_t s) {
   return cudaLaunchKernelEx(&cfg, scored_join_kernel<T>, p, BS, chunk, chunks, row_warps) == cudaSuccess ? VASR_PA_OK : VASR_PA_ELAUNCH;
 }
 
+// Stages of the ring: 32 KB of pages or more in flight a CTA.
+template <typename TC, int BS>
+constexpr int ring_stages() {
+  return 2 * (BS < 16 ? 16 : BS) * kScoredDim * (int)sizeof(TC) <= 8192 ? 8 : 4;
+}
+
+template <typename T, typename TC, int BS, int NRT, bool kDup>
+int launch_mma_rows(const ScoredArgs &a, cudaStream_t s) {
+  constexpr int kNST = ring_stages<TC, BS>(), kMinB = sizeof(TC) == 1 && NRT == 1 ? 4 : 3;
+  static std::atomic<uint64_t> attr_done{0};
+  return launch_split<T, ScoredCfg<TC, BS, kNST>, BS>(a, scored_mma_kernel<T, TC, BS, NRT, kDup, kNST, kMinB>, attr_done,
+                                                      kDup ? 4 : 8 * NRT, s);
+}
+
+template <int BS, int kRows>
+int launch_f32_rows(const ScoredArgs &a, cudaStream_t s) {
+  constexpr int kNST = ring_stages<float, BS>();
+  static std::atomic<uint64_t> attr_done{0};
+  return launch_split<float, ScoredCfg<float, BS, kNST>, BS>(a, scored_f32_kernel<BS, kRows, kNST>, attr_done, kRows, s);
+}
+
+template <int BS>
+int launch_f32_bs(const ScoredArgs &a, cudaStream_t s) {
+  const int rows = a.query_len * (a.num_heads / a.num_kv_heads);
+  if (rows <= 2) return launch_f32_rows<BS, 2>(a, s);
+  if (rows <= 4) return launch_f32_rows<BS, 4>(a, s);
+  return launch_f32_rows<BS, 8>(a, s);
+}
+
 template <typename T, typename TC, int BS>
 int launch_mma_bs(const ScoredArgs &a, cudaStream_t s) {
   const int rows = a.query_len * (a.num_heads / a.num_kv_heads);
@@ -328,8 +355,16 @@ int launch_mma_bs(const ScoredArgs &a, cudaStream_t s) {
 
 template <typename T>
 int launch_scored_c(const ScoredArgs &a, cudaStream_t s) {
-  if constexpr (!std::is_same<T, float>::value) {
-    if (takes_mma(a)) {
+  if constexpr (std::is_same<T, float>::value) {
+    if (takes_split(a)) {
+      switch (a.block_size) {
+        case 8: return launch_f32_bs<8>(a, s);
+        case 16: return launch_f32_bs<16>(a, s);
+        default: return launch_f32_bs<32>(a, s);
+      }
+    }
+  } else {
+    if (takes_split(a)) {
       if (a.cache_dtype == VASR_PA_FP8_E4M3)
         return a.block_size == 16 ? launch_mma_bs<T, __nv_fp8_e4m3, 16>(a, s) : launch_mma_bs<T, __nv_fp8_e4m3, 32>(a, s);
       switch (a.block_size) {
@@ -349,7 +384,7 @@ size_t scored_workspace_bytes(int num_seqs, int query_len, int score_rows, int n
                               int head_dim, int block_size, int max_context_len) {
   const size_t mma =
       head_dim == kScoredDim
-          ? mma_layout(num_seqs, query_len, score_rows, num_heads, num_kv_heads, block_size, max_context_len).total
+          ? split_layout(num_seqs, query_len, score_rows, num_heads, num_kv_heads, block_size, max_context_len).total
           : 0;
   const size_t other = layout(num_seqs, query_len, score_rows, num_heads, head_dim, max_context_len).total;
   return mma > other ? mma : other;
