@@ -207,8 +207,8 @@ __device__ __forceinline__ void move_unit(const E *src, E *dst, int count, bool 
   }
 }
 
-template <typename U, int BS>
-__global__ void __launch_bounds__(kMoveMostThreads) evict_move_kernel(const EvictArgs p) {
+template <typename U, int BS, int kThreads>
+__global__ void __launch_bounds__(kThreads, kThreads == kMoveThreads ? 4 : 1) evict_move_kernel(const EvictArgs p) {
   constexpr int kX = 16 / (int)sizeof(U), kRows = v_rows<U>();
   pdl_wait();
   const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(kMoveMostThreads) evict_move_kernel(const Evic
   const int32_t *kept = p.kept + ((int64_t)b * p.num_kv_heads + h) * p.budget;
   const int D = p.head_dim, chunks = D / kX;
   const int k_units = (chunks + kBatch - 1) / kBatch, units = k_units + (D + kRows - 1) / kRows + 1;
-  for (int r0 = 0; r0 < q.budget; r0 += blockDim.x) {
+  for (int r0 = 0; r0 < q.budget; r0 += kThreads) {
     const int r = r0 + tid;
     int64_t from = -1, to = -1;  // (block, head)
     int so = 0, dof = 0;
@@ -264,14 +264,18 @@ int launch_move_bs(const EvictArgs &a, cudaStream_t s) {
   parts = parts > units ? units : parts;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)parts, (unsigned)a.num_kv_heads, (unsigned)a.num_seqs);
-  cfg.blockDim = dim3(pairs * parts < kMoveCtas / 4 && a.budget > kMoveThreads ? kMoveMostThreads : kMoveThreads);
+  const bool wide = pairs * parts < kMoveCtas / 4 && a.budget > kMoveThreads;
+  cfg.blockDim = dim3(wide ? kMoveMostThreads : kMoveThreads);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, evict_move_kernel<U, BS>, a) == cudaSuccess ? VASR_PA_OK : VASR_PA_ELAUNCH;
+  return cudaLaunchKernelEx(&cfg, wide ? evict_move_kernel<U, BS, kMoveMostThreads> : evict_move_kernel<U, BS, kMoveThreads>, a) ==
+                 cudaSuccess
+             ? VASR_PA_OK
+             : VASR_PA_ELAUNCH;
 }
 
 template <typename U>

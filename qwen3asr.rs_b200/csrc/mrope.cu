@@ -34,14 +34,6 @@ __device__ __forceinline__ int64_t position_of(const MropeAngles &r, int64_t t, 
   return pos < 0 ? 0 : r.max_position - 1;
 }
 
-// d = a b for two f32 pairs, one packed instruction
-__device__ __forceinline__ void mul2(float &d0, float &d1, float a0, float a1, float b0, float b1) {
-  asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
-      "mul.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
-      : "=f"(d0), "=f"(d1)
-      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
-}
-
 // cos and sin of frequency i for token t.
 __device__ __forceinline__ float2 angle_of(const MropeAngles &r, int64_t t, int i) {
   const int64_t at = position_of(r, t, axis_of(r, i)) * r.half + i;
