@@ -31,11 +31,9 @@
 namespace vasr {
 namespace {
 
-constexpr int kRowElems = 64;   // logits a thread of the first launch keeps (32 for f32: 16 vectors)
+constexpr int kRowElems = 32;   // logits a thread of the first launch keeps
 constexpr int kEmitElems = 16;  // logits, drafter's values and noise each that one of the second's does
 constexpr int kMaxThreads = 256;
-template <typename T>
-constexpr int row_elems() { return sizeof(T) == 4 ? kRowElems / 2 : kRowElems; }
 
 // One chunk of a row: its maximum (and, for greedy rows, the first place of
 // it) and sum over the chunk of exp((x - max) / T).
@@ -176,14 +174,14 @@ __device__ __forceinline__ void each_of_group(const Held<T, kGroups> &x, int k, 
 template <typename T>
 __global__ void __launch_bounds__(kMaxThreads) verify_rows_kernel(const VerifyArgs p) {
   pdl_launch_dependents();
-  constexpr int kGroups = row_elems<T>() / kGroup;
+  constexpr int kGroups = kRowElems / kGroup;
   __shared__ float2 part[kMaxThreads / 32];
   __shared__ uint32_t s_arg;
   const int chunk = blockIdx.x, i = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, threads = blockDim.x;
   const int warp = tid >> 5, lane = tid & 31, warps = threads >> 5;
   if (i > drafts_of(p, b)) return;
   const float t = temperature_of(p, b);
-  const int size = threads * row_elems<T>();
+  const int size = threads * kRowElems;
   const int64_t lo = (int64_t)chunk * size;
   const int len = (int)min((int64_t)size, p.vocab - lo);
   Held<T, kGroups> x;
@@ -436,11 +434,11 @@ struct VerifyLayout {
   size_t off_stats, off_verdicts, off_bests, total;
 };
 constexpr size_t kCounterBytes = 65536 * sizeof(uint32_t);  // one per sequence, left at zero
-VerifyLayout verify_layout(int num_seqs, int num_drafts, int64_t vocab, int row_elems) {
+VerifyLayout verify_layout(int num_seqs, int num_drafts, int64_t vocab) {
   VerifyLayout l;
   l.threads = chunk_threads(num_seqs, num_drafts, vocab);
   auto chunks = [&](int elems) { return (int)((vocab + l.threads * elems - 1) / (l.threads * elems)); };
-  l.row_chunks = chunks(row_elems);
+  l.row_chunks = chunks(kRowElems);
   l.emit_chunks = chunks(kEmitElems);
   l.off_stats = kCounterBytes;
   l.off_verdicts = l.off_stats + (size_t)num_seqs * (num_drafts + 1) * l.row_chunks * sizeof(ChunkStat);
@@ -451,7 +449,7 @@ VerifyLayout verify_layout(int num_seqs, int num_drafts, int64_t vocab, int row_
 
 template <typename T, typename TQ>
 int launch_verify_tq(VerifyArgs a, cudaStream_t s) {
-  const VerifyLayout l = verify_layout(a.num_seqs, a.num_drafts, a.vocab, row_elems<T>());
+  const VerifyLayout l = verify_layout(a.num_seqs, a.num_drafts, a.vocab);
   unsigned char *ws = static_cast<unsigned char *>(a.workspace);
   a.counters = reinterpret_cast<uint32_t *>(ws);
   a.stats = ws + l.off_stats;
@@ -491,7 +489,7 @@ int launch_verify_t(const VerifyArgs &a, cudaStream_t s) {
 }  // namespace
 
 size_t verify_workspace_bytes(int num_seqs, int num_drafts, int64_t vocab) {
-  return verify_layout(num_seqs, num_drafts, vocab, kRowElems / 2).total;  // the most chunks of any type
+  return verify_layout(num_seqs, num_drafts, vocab).total;
 }
 
 int launch_verify(const VerifyArgs &a, cudaStream_t s) {
