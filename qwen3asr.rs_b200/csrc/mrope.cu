@@ -226,7 +226,7 @@ constexpr int tile_warps(bool prompt) {
 // Prompts: the part's heads of the tile's rows arrive by one bulk copy a token
 // (a token's heads are adjacent), so that the bytes in flight cost shared
 // memory and not registers; rows are 16 bytes apart modulo 128 to spread banks.
-constexpr int kPartBytes = 2048;  // of one token's row
+constexpr int kPartBytes = 1280;  // of one token's row at most
 template <typename T, int D>
 constexpr int part_heads() { return kPartBytes / (D * (int)sizeof(T)) > 0 ? kPartBytes / (D * (int)sizeof(T)) : 1; }
 template <typename T, int D>
@@ -258,21 +258,22 @@ __global__ void __launch_bounds__(32 * tile_warps<T, D>(kPrompt)) mrope_append_t
   const int part = is_v ? blockIdx.y - qk_parts : blockIdx.y, parts = is_v ? gridDim.y - qk_parts : qk_parts;
   const int heads = is_v ? p.num_kv_heads : p.num_heads + p.num_kv_heads;
   // prompts: a part has its heads [h0, h1) in shared memory; else they are dealt out
-  constexpr int kPartHeads = part_heads<T, D>(), kPitch = part_pitch<T, D>();
-  const int h0 = kPrompt ? part * kPartHeads : 0, h1 = kPrompt ? min(heads, h0 + kPartHeads) : heads;
+  constexpr int kPitch = part_pitch<T, D>();
+  const int per = (heads + parts - 1) / parts;
+  const int h0 = kPrompt ? part * per : 0, h1 = kPrompt ? min(heads, h0 + per) : heads;
   extern __shared__ __align__(128) unsigned char rows[];
   __shared__ __align__(8) uint64_t s_bar;
   if constexpr (kPrompt) {
     const uint32_t bar = smem_addr(&s_bar);
     const int ntok = (int)min((int64_t)kTile, p.num_tokens - tile0);
-    const uint32_t bytes = (uint32_t)((h1 - h0) * D * (int)sizeof(T));
+    const uint32_t bytes = (uint32_t)(max(h1 - h0, 0) * D * (int)sizeof(T));
     if (threadIdx.x == 0) {
       mbar_init(bar, 1);
       mbar_fence_init();
       mbar_arrive_expect_tx(bar, ntok * bytes);
     }
     __syncthreads();
-    if ((int)threadIdx.x < ntok)
+    if ((int)threadIdx.x < ntok && bytes > 0)
       bulk_g2s(smem_addr(rows) + threadIdx.x * kPitch,
                static_cast<const T *>(p.qkv) + (tile0 + threadIdx.x) * p.qkv_token_stride +
                    (int64_t)((is_v ? p.num_heads + p.num_kv_heads : 0) + h0) * D,
