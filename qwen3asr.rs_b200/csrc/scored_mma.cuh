@@ -37,6 +37,9 @@ __global__ void __launch_bounds__(kScoredThreads, MINB) scored_mma_kernel(const 
   using TM = typename std::conditional<kFp8, __half, T>::type;  // MMA operand type
   constexpr int D = C::D, kKS = D / 16, kRows = kDup ? 4 : 8 * NRT;
   constexpr float kRescale = 8.f;  // the running maximum moves when a tile's exceeds it by 2^8
+  // P is 2^(x - m + kLift): in f16 it then fills the range up to 2^15, and
+  // weights down to 2^-31 of the largest are not lost
+  constexpr float kLift = std::is_same<TM, __half>::value ? 7.f : 0.f;
   static_assert(!kDup || NRT == 1, "doubled rows fill one tile of 8");
   extern __shared__ __align__(128) unsigned char smem[];
   pdl_launch_dependents();
@@ -202,7 +205,7 @@ __global__ void __launch_bounds__(kScoredThreads, MINB) scored_mma_kernel(const 
             o[t][j][3] *= a1;
           }
         }
-        const float off = m_used[t] == -INFINITY ? 0.f : m_used[t];
+        const float off = m_used[t] == -INFINITY ? 0.f : m_used[t] - kLift;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           pv[t][e] = scored_exp2(x[e] - off);
@@ -311,7 +314,7 @@ __global__ void __launch_bounds__(kScoredThreads, MINB) scored_mma_kernel(const 
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     if (tig == 0 && !(kDup && grp >= 4))
-      cml[warp * 16 + 8 * t + grp] = aborted ? make_float2(-INFINITY, 0.f) : make_float2(m_used[t], l);
+      cml[warp * 16 + 8 * t + grp] = aborted ? make_float2(-INFINITY, 0.f) : make_float2(m_used[t] - kLift, l);
 #pragma unroll
     for (int j = 0; j < D / 16; ++j)
 #pragma unroll

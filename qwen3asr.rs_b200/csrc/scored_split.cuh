@@ -450,10 +450,14 @@ __global__ void __launch_bounds__(kScoredThreads, 10) scored_join_kernel(const S
   const int n = scored_context(p, b, bs, false);
   const int n_splits = scored_splits(n, p.pages_per_split, bs);
   const int64_t pair = (int64_t)b * p.num_kv_heads + kvh;
-  if (n_splits == 0 || (n_splits == 1 && p.row_tiles == 1)) return;
+  const int j0 = blockIdx.x * chunk, j1 = min(n, j0 + chunk);
+  if (n_splits == 0 || (n_splits == 1 && p.row_tiles == 1) || ((int)blockIdx.x < chunks && j0 >= n)) {
+    // nothing to do; but a grid of which no CTA waited could end, and let the
+    // stream go on, before the split kernel has
+    if (blockIdx.x == 0 && kvh == 0 && b == 0) pdl_wait();
+    return;
+  }
   if ((int)blockIdx.x < chunks) {
-    const int j0 = blockIdx.x * chunk, j1 = min(n, j0 + chunk);
-    if (j0 >= n) return;
     const float *x = p.ws_x + pair * p.scored_rows * p.x_stride;
     pdl_wait();
     ScoredWeights weights;

@@ -199,3 +199,53 @@ def test_ids_and_lengths_out_of_range(cuda_device):
     ctx[1] = 1000                                                # past the table and the bound
     eviction.paged_attention_scored(q, None, None, kc, vc, scores, bt, ctx, 64, 0.1)
     assert pa.device_error() & _lib.DERR_CTX_RANGE
+
+
+@pytest.mark.parametrize("dtype,cache", [(torch.float16, torch.float16), (torch.bfloat16, FP8), (torch.float16, FP8)])
+def test_many_small_weights_beside_a_large_one(cuda_device, dtype, cache):
+    """One token 2^20 times as heavy as each of 6000 others, whose values all point one way: weights
+    far below f16's smallest value next to the largest still reach the output."""
+    dev, n, d, bs = cuda_device, 6001, 128, 16
+    rng = np.random.default_rng(20)
+    kc, vc, tables = ref.make_pool(rng, (n,), 1, d, bs, cache, dev, fill=False)
+    k = torch.zeros(kc.shape[0] * bs, 1, d)
+    v = torch.full((kc.shape[0] * bs, 1, d), 400.0)
+    sl = ref.slots_of(tables[0], n, bs)
+    k[sl[0], 0, 0] = 1.0
+    v[sl[0]] = 0.0
+    x = kc.shape[-1]
+    kc = k.view(-1, bs, 1, d // x, x).permute(0, 2, 3, 1, 4).contiguous().to(cache).to(dev)
+    vc = v.view(-1, bs, 1, d).permute(0, 2, 3, 1).contiguous().to(cache).to(dev)
+    q = torch.zeros(1, 1, 2, d, dtype=dtype, device=dev)
+    q[..., 0] = 20 * float(np.log(2.0))
+    scores = torch.zeros(kc.shape[0], 1, bs, device=dev)
+    one = torch.ones(1, device=dev) if cache == FP8 else None
+    out = eviction.paged_attention_scored(q, one, one, kc, vc, scores, torch.from_numpy(tables).to(dev),
+                                          torch.tensor([n], dtype=torch.int32, device=dev), n, 1.0)
+    want, _, _, reach = ref.scored(q, kc, vc, torch.zeros_like(scores), tables, (n,), 1.0)
+    # P to 11 bits, or to f16's spacing of 2^-31 of the largest weight; V 400, the sum of weights near 1
+    rel = 128 * 2.0 ** -23 * reach + 2.0 ** -18
+    tol = (ref.ROUND[dtype] + 2.0 ** -11 + rel) * want + 6000 * 2.0 ** -32 * 400
+    assert (want > 1).all() and (np.abs(ref.f64(out) - want) <= tol).all()
+
+
+def test_loose_bound_leaves_the_order_of_the_stream(cuda_device):
+    """Contexts of one split under a bound of many: the join has nothing to do, and what follows on
+    the stream still sees the finished output and scores."""
+    dev = cuda_device
+    rng = np.random.default_rng(21)
+    lens = [900] * 64
+    kc, vc, tables = ref.make_pool(rng, lens, 8, 128, 16, torch.bfloat16, dev, extra_cols=200)
+    q = torch.from_numpy(rng.standard_normal((64, 16, 128), np.float32)).to(torch.bfloat16).to(dev)
+    bt = torch.from_numpy(tables).to(dev)
+    ctx = torch.tensor(lens, dtype=torch.int32, device=dev)
+    got = []
+    for _ in range(20):
+        s = torch.zeros(kc.shape[0], 8, 16, device=dev)
+        out = eviction.paged_attention_scored(q, None, None, kc, vc, s, bt, ctx, 4000, 128 ** -0.5)
+        got.append((out.clone(), s.clone()))  # ordered behind the call by the stream alone
+    torch.cuda.synchronize()
+    for out, s in got[1:]:
+        assert torch.equal(out, got[0][0]) and torch.equal(s, got[0][1])
+    # the 16 query heads' weights of every sequence sum to 16
+    assert abs(float(got[-1][1].double().sum()) - 64 * 16) < 64 * 16 * 1e-4
