@@ -6,6 +6,8 @@
 * ``lib/_vasr_host*.so`` — the C++ host mirror of the ``vasr-paged-attn``
   Rust API (metadata builders, block manager, graph buckets) as a pybind11
   module, used by the Python package and the tests.
+* ``lib/_vasr_calls*.so`` — the tensor-level entry points whose host cost counts
+  (g++ against torch's headers); the kernels stay in ``libvasr_pa.so``.
 
 Objects go to ``_build/``; each unit is rebuilt only when it or a header it
 may include is newer than its object. Run ``python build.py`` or call
@@ -112,9 +114,33 @@ def build_host() -> Path | None:
     return out
 
 
+def build_calls() -> Path:
+    """Compile the torch extension module of ``csrc/torch`` (no link to the kernels: it is bound to
+    the loaded library at run time)."""
+    import torch  # noqa: PLC0415
+
+    LIB.mkdir(exist_ok=True)
+    out = LIB / f"_vasr_calls{sysconfig.get_config_var('EXT_SUFFIX') or '.so'}"
+    src = CSRC / "torch" / "tensor_calls.cpp"
+    if not _stale(out, [src], (INCLUDE / "vasr_pa.h").stat().st_mtime):
+        return out
+    root = Path(torch.__file__).resolve().parent
+    _run([
+        shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall", "-fvisibility=hidden",
+        f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", str(INCLUDE),
+        "-isystem", str(root / "include"), "-isystem", str(root / "include" / "torch" / "csrc" / "api" / "include"),
+        "-isystem", sysconfig.get_paths()["include"], "-isystem", str(CUDA_HOME / "include"), str(src), "-o", str(out),
+        "-L", str(root / "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
+    ])
+    return out
+
+
 def build(verbose: bool = False) -> None:
-    build_cuda(verbose=verbose)
-    build_host()
+    with cf.ThreadPoolExecutor(max_workers=2) as ex:
+        calls = ex.submit(build_calls)
+        build_cuda(verbose=verbose)
+        build_host()
+        calls.result()
 
 
 if __name__ == "__main__":

@@ -58,19 +58,6 @@ def _require_cuda(*tensors: torch.Tensor) -> torch.device:
     return dev
 
 
-def _cuda_index(*tensors: torch.Tensor) -> int:
-    """The tensors' common CUDA device (``_require_cuda`` for calls short enough that its cost counts)."""
-    dev = tensors[0].get_device()
-    for t in tensors:
-        if t.get_device() != dev or dev < 0:
-            _require_cuda(*tensors)
-    return dev
-
-
-# the current stream's handle by device index, without building a Stream object
-_raw_stream = torch._C._cuda_getCurrentRawStream
-
-
 def cache_geometry(key_cache: torch.Tensor, value_cache: torch.Tensor):
     """(num_blocks, num_kv_heads, head_dim, block_size) of a vLLM-layout cache pair."""
     if key_cache.dim() != 5 or value_cache.dim() != 4:
@@ -154,30 +141,6 @@ def reserve_paged_attention_workspace(device: torch.device, nbytes: int,
         ws = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
         _WORKSPACES[key] = ws
     return ws
-
-
-class StreamWorkspaces:
-    """One growing, zero-filled workspace per (device, stream) for one kind of call."""
-
-    def __init__(self, what: str):
-        self._what = what
-        self._held: dict[tuple[int, int], torch.Tensor] = {}
-
-    def reserve(self, device: int, stream: int, nbytes: int) -> torch.Tensor:
-        """The workspace of a stream (its handle), at least ``nbytes`` long."""
-        ws = self._held.get((device, stream))
-        if ws is None or ws.numel() < nbytes:
-            if torch.cuda.is_current_stream_capturing():
-                raise _lib.VasrPaError(_lib.EINVAL_WORKSPACE,
-                                       f"{self._what} workspace must be reserved before CUDA graph capture")
-            ws = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=torch.device("cuda", device))
-            self._held[(device, stream)] = ws
-        return ws
-
-    def reserve_for(self, device, nbytes: int, stream: Optional[torch.cuda.Stream]) -> torch.Tensor:
-        device = torch.device(device)
-        s = stream if stream is not None else torch.cuda.current_stream(device)
-        return self.reserve(s.device.index, s.cuda_stream, nbytes)
 
 
 _PREFILL_SCRATCH: dict[tuple[int, int], torch.Tensor] = {}
