@@ -23,6 +23,15 @@
 // has its noise in registers by the time the verdict is there, and the last
 // CTA of a sequence takes the winner. Only the row that is drawn from is read
 // twice, the second time from L2.
+//
+// A large call is bound by memory and, nearly as much, by the exponentials: 64
+// sequences of 5 bf16 rows of 151936 logits with an f32 drafter take 47 us for
+// the 175 MB that must be read (3.7 TB/s), 32 x 8 f32 rows without a drafter
+// 40 us (4.4 TB/s). One sequence takes 8.9 us, the latency of three launches
+// that each wait for one round of loads; CTAs of 64 threads, four times as
+// many, took 11.7 us there (more chunks to join) and 52 us for the large call.
+// CTAs that stay and load the next chunk ahead of the current one's work need
+// registers for two, and were slower (50 us).
 #include <type_traits>
 
 #include "common.cuh"
@@ -31,9 +40,9 @@
 namespace vasr {
 namespace {
 
-constexpr int kRowElems = 32;   // logits a thread of the first launch keeps
-constexpr int kEmitElems = 16;  // logits, drafter's values and noise each that one of the second's does
-constexpr int kMaxThreads = 256;
+constexpr int kThreads = 256;
+constexpr int kRowElems = 32;   // logits a thread of the first launch keeps (16: 49 us for the large call)
+constexpr int kEmitElems = 16;  // of logits, drafter's values and noise each, in the third (8: 59 us, 32: 48 us)
 
 // One chunk of a row: its maximum (and, for greedy rows, the first place of
 // it) and sum over the chunk of exp((x - max) / T).
@@ -103,12 +112,12 @@ struct Held {
   static constexpr int kVec = 16 / (int)sizeof(T);
   static constexpr int kVecs = kGroup / kVec;
   uint4 raw[kGroups][kVecs];
-  __device__ __forceinline__ void load(const T *row, int len, int tid, int threads) {
+  __device__ __forceinline__ void load(const T *row, int len, int tid) {
     const bool aligned = reinterpret_cast<uintptr_t>(row) % 16 == 0;
 #pragma unroll
     for (int k = 0; k < kGroups; ++k) {
-      const int j = (tid + k * threads) * kGroup;
-      if (aligned && (k + 1) * threads * kGroup <= len) {  // the whole CTA's groups
+      const int j = (tid + k * kThreads) * kGroup;
+      if (aligned && (k + 1) * kThreads * kGroup <= len) {  // the whole CTA's groups
 #pragma unroll
         for (int v = 0; v < kVecs; ++v) raw[k][v] = __ldg(reinterpret_cast<const uint4 *>(row + j) + v);
       } else {
@@ -160,8 +169,8 @@ struct Held {
 // f(value, index) for the thread's elements of group k that lie in the chunk
 // and are not NaN; groups past a chunk's end have none.
 template <typename T, int kGroups, typename F>
-__device__ __forceinline__ void each_of_group(const Held<T, kGroups> &x, int k, int len, int tid, int threads, F f) {
-  const int j = (tid + k * threads) * kGroup;
+__device__ __forceinline__ void each_of_group(const Held<T, kGroups> &x, int k, int len, int tid, F f) {
+  const int j = (tid + k * kThreads) * kGroup;
   if (j >= len) return;
   float v[kGroup];
   x.group(k, v);
@@ -172,27 +181,27 @@ __device__ __forceinline__ void each_of_group(const Held<T, kGroups> &x, int k, 
 
 // grid = (chunk, row, sequence)
 template <typename T>
-__global__ void __launch_bounds__(kMaxThreads) verify_rows_kernel(const VerifyArgs p) {
+__global__ void __launch_bounds__(kThreads) verify_rows_kernel(const VerifyArgs p) {
   pdl_launch_dependents();
   constexpr int kGroups = kRowElems / kGroup;
-  __shared__ float2 part[kMaxThreads / 32];
+  __shared__ float2 part[kThreads / 32];
   __shared__ uint32_t s_arg;
-  const int chunk = blockIdx.x, i = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, threads = blockDim.x;
-  const int warp = tid >> 5, lane = tid & 31, warps = threads >> 5;
+  const int chunk = blockIdx.x, i = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+  const int warp = tid >> 5, lane = tid & 31, warps = kThreads >> 5;
   if (i > drafts_of(p, b)) return;
   const float t = temperature_of(p, b);
-  const int size = threads * kRowElems;
+  const int size = kThreads * kRowElems;
   const int64_t lo = (int64_t)chunk * size;
   const int len = (int)min((int64_t)size, p.vocab - lo);
   Held<T, kGroups> x;
-  x.load(static_cast<const T *>(p.logits) + b * p.logits_seq_stride + i * p.logits_row_stride + lo, len, tid, threads);
+  x.load(static_cast<const T *>(p.logits) + b * p.logits_seq_stride + i * p.logits_row_stride + lo, len, tid);
   // the thread's own maximum and sum, then the warp's, then the chunk's
-  const int whole = len / (threads * kGroup);  // groups that all threads have
+  const int whole = len / (kThreads * kGroup);  // groups that all threads have
   float m = -INFINITY, sum = 0.f;
 #pragma unroll
   for (int g = 0; g < kGroups; ++g) {
     if (g < whole) m = fmaxf(m, x.group_max(g));
-    else each_of_group(x, g, len, tid, threads, [&](float v, int) { m = fmaxf(m, v); });
+    else each_of_group(x, g, len, tid, [&](float v, int) { m = fmaxf(m, v); });
   }
   const float c = kLog2e / t;
   if (t > 0.f && m > -INFINITY) {
@@ -204,14 +213,14 @@ __global__ void __launch_bounds__(kMaxThreads) verify_rows_kernel(const VerifyAr
 #pragma unroll
         for (int e = 0; e < kGroup; ++e) sum += plain_weight(v[e], m, c);
       } else {
-        each_of_group(x, g, len, tid, threads, [&](float v, int) { sum += weight_of(v, m, c); });
+        each_of_group(x, g, len, tid, [&](float v, int) { sum += weight_of(v, m, c); });
       }
     }
     if (!(sum == sum)) {  // an infinite maximum or a NaN among the logits
       sum = 0.f;
 #pragma unroll
       for (int g = 0; g < kGroups; ++g)
-        each_of_group(x, g, len, tid, threads, [&](float v, int) { sum += weight_of(v, m, c); });
+        each_of_group(x, g, len, tid, [&](float v, int) { sum += weight_of(v, m, c); });
     }
   }
   const float wm = warp_max_xor(m, 32);
@@ -227,7 +236,7 @@ __global__ void __launch_bounds__(kMaxThreads) verify_rows_kernel(const VerifyAr
     uint32_t first = kNone;
 #pragma unroll
     for (int g = 0; g < kGroups; ++g)
-      each_of_group(x, g, len, tid, threads, [&](float v, int j) {
+      each_of_group(x, g, len, tid, [&](float v, int j) {
         if (v == cm) first = min(first, (uint32_t)j);
       });
     if (first != kNone) atomicMin(&s_arg, first);
@@ -264,7 +273,7 @@ __device__ __forceinline__ ChunkStat join_chunks(const VerifyArgs &p, int64_t ro
 
 // One CTA per sequence: every row's sum, then the verdict.
 template <typename T, typename TQ>
-__global__ void __launch_bounds__(kMaxThreads) verify_verdict_kernel(const VerifyArgs p) {
+__global__ void __launch_bounds__(kThreads) verify_verdict_kernel(const VerifyArgs p) {
   pdl_launch_dependents();
   extern __shared__ ChunkStat s_row[];  // [num_drafts + 1]
   __shared__ int s_fail;
@@ -316,18 +325,18 @@ __global__ void __launch_bounds__(kMaxThreads) verify_verdict_kernel(const Verif
 
 // grid = (chunk, sequence)
 template <typename T, typename TQ>
-__global__ void __launch_bounds__(kMaxThreads, 4) verify_emit_kernel(const VerifyArgs p) {
+__global__ void __launch_bounds__(kThreads, 4) verify_emit_kernel(const VerifyArgs p) {
   constexpr int kGroups = kEmitElems / kGroup;
-  __shared__ Best part[kMaxThreads / 32];
-  const int chunk = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, threads = blockDim.x;
-  const int warp = tid >> 5, lane = tid & 31, warps = threads >> 5;
+  __shared__ Best part[kThreads / 32];
+  const int chunk = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+  const int warp = tid >> 5, lane = tid & 31, warps = kThreads >> 5;
   const float t = temperature_of(p, b);
-  const int size = threads * kEmitElems;
+  const int size = kThreads * kEmitElems;
   const int64_t lo = (int64_t)chunk * size;
   const int len = (int)min((int64_t)size, p.vocab - lo);
   // inputs come early, while the launches before still run
   Held<float, kGroups> race;
-  if (t > 0.f) race.load(p.race + b * p.race_seq_stride + lo, len, tid, threads);
+  if (t > 0.f) race.load(p.race + b * p.race_seq_stride + lo, len, tid);
   const int k = drafts_of(p, b);
   pdl_wait();
   const float4 raw = __ldcg(static_cast<const float4 *>(p.verdicts) + b);
@@ -338,12 +347,11 @@ __global__ void __launch_bounds__(kMaxThreads, 4) verify_emit_kernel(const Verif
   // ---- the race over this chunk. The quotient takes one reciprocal
   // instruction (1 ulp); only r / e > 0 can win, so NaN and r <= 0 drop out.
   Held<T, kGroups> x;
-  x.load(row + lo, len, tid, threads);
+  x.load(row + lo, len, tid);
   const bool with_q = p.draft_probs && s.n < k;
   Held<TQ, kGroups> q;
   if (with_q)
-    q.load(static_cast<const TQ *>(p.draft_probs) + b * p.probs_seq_stride + s.n * p.probs_row_stride + lo, len, tid,
-           threads);
+    q.load(static_cast<const TQ *>(p.draft_probs) + b * p.probs_seq_stride + s.n * p.probs_row_stride + lo, len, tid);
   int skip = -1;  // a failed draft that the drafter was certain of
   if (s.n < k && !with_q) {
     const int64_t failed = (int64_t)p.draft_tokens[(int64_t)b * p.num_drafts + s.n] - lo;
@@ -354,7 +362,7 @@ __global__ void __launch_bounds__(kMaxThreads, 4) verify_emit_kernel(const Verif
   int place = -1;  // g * 8 + i of the winner
 #pragma unroll
   for (int g = 0; g < kGroups; ++g) {
-    const int j = (tid + g * threads) * kGroup;
+    const int j = (tid + g * kThreads) * kGroup;
     float w[kGroup], e[kGroup], qv[kGroup];
     x.group(g, w);
     race.group(g, e);
@@ -385,7 +393,7 @@ __global__ void __launch_bounds__(kMaxThreads, 4) verify_emit_kernel(const Verif
     }
   }
   Best best{top, kNone};
-  if (place >= 0) best.i = (uint32_t)(lo + (tid + place / kGroup * threads) * kGroup + place % kGroup);
+  if (place >= 0) best.i = (uint32_t)(lo + (tid + place / kGroup * kThreads) * kGroup + place % kGroup);
   best = warp_best(best);
   if (lane == 0) part[warp] = best;
   __syncthreads();
@@ -422,22 +430,14 @@ __global__ void __launch_bounds__(kMaxThreads, 4) verify_emit_kernel(const Verif
   }
 }
 
-// CTAs of 256 threads; calls whose chunks would not fill the SMs take CTAs of
-// 64, which cost more reductions per byte.
-int chunk_threads(int num_seqs, int num_drafts, int64_t vocab) {
-  const int64_t ctas = (int64_t)num_seqs * (num_drafts + 1) * ((vocab + 8191) / 8192);
-  return ctas >= 2 * 148 ? 256 : 64;
-}
-
 struct VerifyLayout {
-  int threads, row_chunks, emit_chunks;
+  int row_chunks, emit_chunks;
   size_t off_stats, off_verdicts, off_bests, total;
 };
 constexpr size_t kCounterBytes = 65536 * sizeof(uint32_t);  // one per sequence, left at zero
 VerifyLayout verify_layout(int num_seqs, int num_drafts, int64_t vocab) {
   VerifyLayout l;
-  l.threads = chunk_threads(num_seqs, num_drafts, vocab);
-  auto chunks = [&](int elems) { return (int)((vocab + l.threads * elems - 1) / (l.threads * elems)); };
+  auto chunks = [&](int elems) { return (int)((vocab + kThreads * elems - 1) / (kThreads * elems)); };
   l.row_chunks = chunks(kRowElems);
   l.emit_chunks = chunks(kEmitElems);
   l.off_stats = kCounterBytes;
@@ -457,7 +457,7 @@ int launch_verify_tq(VerifyArgs a, cudaStream_t s) {
   a.bests = ws + l.off_bests;
   a.row_chunks = l.row_chunks;
   verify_rows_kernel<T><<<dim3((unsigned)l.row_chunks, (unsigned)a.num_drafts + 1, (unsigned)a.num_seqs),
-                          (unsigned)l.threads, 0, s>>>(a);
+                          kThreads, 0, s>>>(a);
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -465,13 +465,13 @@ int launch_verify_tq(VerifyArgs a, cudaStream_t s) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   cfg.stream = s;
-  const int row_warps = a.num_drafts + 1 < kMaxThreads / 32 ? a.num_drafts + 1 : kMaxThreads / 32;
+  const int row_warps = a.num_drafts + 1 < kThreads / 32 ? a.num_drafts + 1 : kThreads / 32;
   cfg.gridDim = dim3((unsigned)a.num_seqs);
   cfg.blockDim = dim3((unsigned)row_warps * 32);
   cfg.dynamicSmemBytes = (size_t)(a.num_drafts + 1) * sizeof(ChunkStat);
   if (cudaLaunchKernelEx(&cfg, verify_verdict_kernel<T, TQ>, a) != cudaSuccess) return VASR_PA_ELAUNCH;
   cfg.gridDim = dim3((unsigned)l.emit_chunks, (unsigned)a.num_seqs);
-  cfg.blockDim = dim3((unsigned)l.threads);
+  cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = 0;
   return cudaLaunchKernelEx(&cfg, verify_emit_kernel<T, TQ>, a) == cudaSuccess ? VASR_PA_OK : VASR_PA_ELAUNCH;
 }
