@@ -537,9 +537,10 @@ int32_t vasr_pa_paged_attention_scored(
  * may be NULL) lowers the budget per sequence; where it is under num_sink +
  * num_recent, the lowest indices of those stay. kept
  * [num_seqs, num_kv_heads, budget] receives the old indices, ascending, then
- * -1; new_lens [num_seqs] = min(context_len, budget). In place, block tables
- * of different sequences must not name the same block. dtype is the pages'
- * element type (fp8 too).
+ * -1; new_lens [num_seqs] = min(context_len, budget), an array other than
+ * context_lens (VASR_PA_EINVAL_POINTER). In place, block tables of different
+ * sequences must not name the same block. dtype is the pages' element type
+ * (fp8 too).
  */
 int32_t vasr_pa_evict_kv(void *key_cache, void *value_cache, float *score_cache,
                          const uint32_t *block_tables, int32_t max_num_blocks_per_seq,

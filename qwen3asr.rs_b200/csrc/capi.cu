@@ -750,6 +750,7 @@ int32_t vasr_pa_evict_kv(void *key_cache, void *value_cache, float *score_cache,
       !aligned(out_block_tables, 4) || !aligned(context_lens, 4) || !aligned(budgets, 4) || !aligned(kept, 4) ||
       !aligned(new_lens, 4))
     return VASR_PA_EINVAL_ALIGN;
+  if (new_lens == context_lens) return VASR_PA_EINVAL_POINTER;  // the old lengths are read until the end
   vasr::EvictArgs a{key_cache, value_cache, score_cache, block_tables, out_block_tables, context_lens, budgets,
                     kept, new_lens, max_context_len, budget, num_sink, num_recent, num_seqs, num_kv_heads,
                     head_dim, block_size, num_blocks, max_num_blocks_per_seq, out_max_num_blocks_per_seq, es};

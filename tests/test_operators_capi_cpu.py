@@ -94,6 +94,12 @@ def test_evict_refusals():
         (dict(kept=ODD), _lib.EINVAL_ALIGN), (dict(b=0), _lib.OK)])
 
 
+def test_evict_refuses_the_lengths_as_their_own_output():
+    base = dict(kc=P, vc=P, scores=P, bt=P, cols=4, obt=None, ocols=0, ctx=P, bound=64, budgets=None, budget=32, sink=4,
+                recent=8, kept=P, lens=P, b=4, hkv=8, d=128, bs=16, nb=10, dtype=_lib.BF16, stream=None)
+    refuse(_lib.lib().vasr_pa_evict_kv, base, [(dict(), _lib.EINVAL_POINTER), (dict(b=0), _lib.OK)])
+
+
 def test_verify_refusals():
     lib = _lib.lib()
     need = lib.vasr_pa_verify_draft_tokens_workspace_size(4, 3, 1000)
