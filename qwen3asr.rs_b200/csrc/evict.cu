@@ -8,21 +8,45 @@
 // its own set, which the page layout allows because a block holds each head's
 // tokens apart.
 //
-// Selection is a radix select over order-preserving keys of the scores, which
-// a CTA per (sequence, kv head) keeps in shared memory; the move copies bits,
-// bound by memory: it reads every 32-byte sector that holds a kept token and
-// writes the kept ones. In place, token r of the result comes from an index
-// >= r, so places filled in ascending tiles never overwrite a token that is
-// still needed, as long as a tile is read before it or a later one is written:
-// a CTA moves its slices of the head dimension of one (sequence, head) that way.
+// Selection is a radix select over order-preserving keys of the scores, kept
+// in shared memory: a histogram of one byte per pass, at most four passes, and
+// a last one that lists the survivors by rank. A CTA has a (sequence, kv head);
+// long contexts of few sequences take a cluster of CTAs, which add their
+// histograms up over distributed shared memory. It is bound by latency: 8
+// heads of 4099 tokens take about 10 us of launch, loads and barriers.
+//
+// The move copies bits, bound by memory: it reads every 32-byte sector that
+// holds a kept token and writes the kept ones. A sector of V holds 16 tokens
+// of one dim (16-bit pages), so that nearly all of V is read whatever stays:
+// 640 of 700 to 1500 tokens of 64 sequences are 342 MB of kept K, V and scores,
+// 428 MB of sectors, and take 94 us with the selection (the move alone 81% of
+// the copy rate in sectors). In place, token r of the result comes from an
+// index >= r, so places filled in ascending tiles never overwrite a token that
+// is still needed, as long as a tile is read before it or a later one is
+// written: a CTA moves its slices of the head dimension of one (sequence,
+// head) that way. Measured slower: tables and indices fetched a tile or two
+// ahead (114 us: the registers cost a fifth of the loads in flight), 6 CTAs an
+// SM (127 us), 8 K chunks or 32 V rows a unit (97 and 99 us), and tiles of one
+// (sequence, head) shared among CTAs when the pages do not overlap (no gain).
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 #include "launch.h"
+
+namespace cg = cooperative_groups;
 
 namespace vasr {
 namespace {
 
 constexpr int kSelectThreads = 512;
-constexpr int kSelectMostThreads = 1024;  // calls of few (sequence, head)s: 16 against 18 us for 8 of 4099 tokens
+constexpr int kSelectMostThreads = 1024;  // at most 148 (sequence, head)s: 16 against 18 us for 8 of 4099 tokens
+// Keys in a CTA's shared memory: 32 KB, or most of an SM's where every CTA has
+// one to itself (one sequence of 32768 tokens, one CTA a head: 62 against 96 us).
+constexpr int kKeys = 8192, kMostKeys = 49152;
+// Longer contexts of up to 74 (sequence, head)s take clusters of up to 8 CTAs:
+// 21 against 26 us at 8 heads of 9000 tokens, 30 / 51 at 20000, 79 / 92 at 32
+// heads of 20000; at 2000 tokens 14.5 / 11.6, at 32 heads of 4099 24 / 22.6.
+constexpr int kClusterTokens = 8192, kMostClusterCtas = 8;
 constexpr int kMoveThreads = 256;
 constexpr int kMoveMostThreads = 1024;
 constexpr int kMoveCtas = 8 * 148;
@@ -62,30 +86,35 @@ __device__ __forceinline__ int64_t block_at(const uint32_t *table, int col, int6
   return -1;
 }
 
-// kept[b, h, :] = the indices that stay, ascending, then -1. key_cap tokens'
-// keys fit the dynamic shared memory; those past them are made anew on every
-// pass.
-template <int kThreads>
+// kept[b, h, :] = the indices that stay, ascending, then -1. The CTAs of a
+// (sequence, head) form a cluster (kCluster; else there is one) and have a
+// stretch of its tokens each; the keys of a stretch's first key_cap tokens fit
+// the dynamic shared memory, those past them are made anew on every pass.
+template <int kThreads, bool kCluster>
 __global__ void __launch_bounds__(kThreads) evict_select_kernel(const EvictArgs p, int key_cap) {
   extern __shared__ uint32_t s_key[];
-  __shared__ int hist[256];
+  __shared__ int s_hist[4][256], s_total[256];  // a pass's own counts, and the cluster's
   __shared__ int s_above[kThreads / 32], s_ties[kThreads / 32];
+  __shared__ int2 s_cta;
   __shared__ uint32_t s_prefix;
   __shared__ int s_rank, s_done;
   pdl_launch_dependents();
-  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int ctas = kCluster ? (int)cluster.num_blocks() : 1, cta = kCluster ? (int)cluster.block_rank() : 0;
+  const int h = blockIdx.x / ctas, b = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int shift = 31 - __clz(p.block_size);
   const Sequence q = sequence_of(p, b);
   int32_t *kept = p.kept + ((int64_t)b * p.num_kv_heads + h) * p.budget;
-  if (h == 0 && tid == 0) p.new_lens[b] = (uint32_t)q.budget;
-  for (int i = q.budget + tid; i < p.budget; i += kThreads) kept[i] = -1;
+  if (blockIdx.x == 0 && tid == 0) p.new_lens[b] = (uint32_t)q.budget;
+  for (int i = q.budget + cta * kThreads + tid; i < p.budget; i += ctas * kThreads) kept[i] = -1;
   if (q.len == q.budget) {
-    for (int i = tid; i < q.budget; i += kThreads) kept[i] = i;
+    for (int i = cta * kThreads + tid; i < q.budget; i += ctas * kThreads) kept[i] = i;
     return;
   }
   if (q.budget == 0) return;
   const uint32_t *table = p.block_tables + (int64_t)b * p.cols;
   const int recent0 = q.len - p.num_recent;
+  const int stretch = (q.len + ctas - 1) / ctas, t0 = min(cta * stretch, q.len), t1 = min(t0 + stretch, q.len);
   auto make_key = [&](int j) -> uint32_t {
     const int64_t blk = block_at(table, j >> shift, p.num_blocks);
     if (j < p.num_sink || j >= recent0) return 0xffffffffu;
@@ -93,22 +122,32 @@ __global__ void __launch_bounds__(kThreads) evict_select_kernel(const EvictArgs 
     return score_key(p.score_cache[((blk * p.num_kv_heads + h) << shift) + (j & (p.block_size - 1))]);
   };
 #pragma unroll 4
-  for (int j = tid; j < min(q.len, key_cap); j += kThreads) s_key[j] = make_key(j);
-  auto key_of = [&](int j) { return j < key_cap ? s_key[j] : make_key(j); };
+  for (int j = tid; j < min(t1 - t0, key_cap); j += kThreads) s_key[j] = make_key(t0 + j);
+  auto key_of = [&](int j) { return j - t0 < key_cap ? s_key[j - t0] : make_key(j); };
+  for (int i = tid; i < 4 * 256; i += kThreads) s_hist[i / 256][i % 256] = 0;
+  __syncthreads();
   // ---- the key of rank `budget` from above, one byte of it per pass
   uint32_t prefix = 0, mask = 0;
   int rank = q.budget;  // 1-based rank among the keys that match the prefix
   for (int shift8 = 24; shift8 >= 0; shift8 -= 8) {
-    if (tid < 256) hist[tid] = 0;
-    __syncthreads();
-    for (int j0 = 0; j0 < q.len; j0 += kThreads) {
+    int *hist = s_hist[shift8 / 8];
+    for (int j0 = t0; j0 < t1; j0 += kThreads) {
       const int j = j0 + tid;
-      const uint32_t key = j < q.len ? key_of(j) : 0u;
-      const bool in = j < q.len && (key & mask) == prefix;
+      const uint32_t key = j < t1 ? key_of(j) : 0u;
+      const bool in = j < t1 && (key & mask) == prefix;
       // one count per distinct digit of the warp: scores share their leading bytes
       const uint32_t digit = in ? (key >> shift8) & 255u : 256u;
       const uint32_t same = __match_any_sync(0xffffffffu, digit);
       if (in && lane == __ffs(same) - 1) atomicAdd(&hist[digit], __popc(same));
+    }
+    if constexpr (kCluster) {
+      cluster.sync();
+      if (tid < 256) {
+        int sum = 0;
+        for (int c = 0; c < ctas; ++c) sum += cluster.map_shared_rank(hist, c)[tid];
+        s_total[tid] = sum;
+      }
+      hist = s_total;
     }
     __syncthreads();
     if (warp == 0) {  // lane l: digits 255 - 8 l downwards; which one holds the rank
@@ -137,9 +176,9 @@ __global__ void __launch_bounds__(kThreads) evict_select_kernel(const EvictArgs 
     if (s_done) break;
   }
   // ---- kept are the keys above the prefix and the first `rank` equal to it:
-  // each warp counts its stretch of the tokens, then writes it
-  const int per = (q.len + kThreads - 1) / kThreads * 32;  // tokens of a warp
-  const int j0 = warp * per, j1 = min(q.len, j0 + per);
+  // each warp counts its part of the stretch, then writes it
+  const int per = (t1 - t0 + kThreads - 1) / kThreads * 32;  // tokens of a warp
+  const int j0 = t0 + warp * per, j1 = min(t1, j0 + per);
   int above = 0, ties = 0;
   for (int j = j0 + lane; j < j1; j += 32) {
     const uint32_t key = key_of(j);
@@ -154,6 +193,18 @@ __global__ void __launch_bounds__(kThreads) evict_select_kernel(const EvictArgs 
   }
   __syncthreads();
   above = ties = 0;
+  if constexpr (kCluster) {  // what the cluster's lower CTAs have
+    if (warp == 0) {
+      const int up = __reduce_add_sync(0xffffffffu, lane < kThreads / 32 ? s_above[lane] : 0);
+      const int eq = __reduce_add_sync(0xffffffffu, lane < kThreads / 32 ? s_ties[lane] : 0);
+      if (lane == 0) s_cta = make_int2(up, eq);
+    }
+    cluster.sync();
+    const int2 lower_cta = lane < cta ? *cluster.map_shared_rank(&s_cta, lane) : make_int2(0, 0);
+    above = __reduce_add_sync(0xffffffffu, lower_cta.x);
+    ties = __reduce_add_sync(0xffffffffu, lower_cta.y);
+    cluster.barrier_arrive();  // this CTA has read the others' shared memory
+  }
   for (int w = 0; w < warp; ++w) {
     above += s_above[w];
     ties += s_ties[w];
@@ -169,6 +220,7 @@ __global__ void __launch_bounds__(kThreads) evict_select_kernel(const EvictArgs 
     above += __popc(ups);
     ties += __popc(eqs);
   }
+  if constexpr (kCluster) cluster.barrier_wait();
 }
 
 // The move of one (sequence, head), in units that gridDim.x CTAs share: kBatch
@@ -255,7 +307,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == kMoveThreads ? 4 : 1) ev
 }
 
 // CTAs per (sequence, head): enough to fill the SMs, at most one per unit.
-// Where even that leaves SMs idle, tiles of 1024 tokens take fewer turns.
+// Where even that leaves most SMs' places empty, tiles of 1024 tokens take fewer
+// turns: 15.9 against 17.3 us at one sequence of 4099 tokens, 62 / 70 at 32768.
 template <typename U, int BS>
 int launch_move_bs(const EvictArgs &a, cudaStream_t s) {
   const int chunks = a.head_dim * (int)sizeof(U) / 16;
@@ -291,19 +344,35 @@ int launch_move(const EvictArgs &a, cudaStream_t s) {
 }  // namespace
 
 int launch_evict(const EvictArgs &a, cudaStream_t s) {
-  // keys in shared memory: 32 KB a CTA, or most of an SM's where there are few CTAs
-  constexpr int kMostKeys = 49152;
   const int64_t pairs = (int64_t)a.num_seqs * a.num_kv_heads;
-  int key_cap = a.max_context_len < 8192 || pairs > 148 ? 8192 : kMostKeys;
-  if (key_cap > a.max_context_len) key_cap = a.max_context_len;
-  const dim3 grid((unsigned)a.num_kv_heads, (unsigned)a.num_seqs);
-  if (pairs <= 148) {
-    auto kern = evict_select_kernel<kSelectMostThreads>;
-    static std::atomic<uint64_t> attr_done{0};
-    if (!ensure_smem_attr(kern, kMostKeys * 4, attr_done)) return VASR_PA_ELAUNCH;
-    kern<<<grid, kSelectMostThreads, key_cap * 4, s>>>(a, key_cap);
-  } else {  // at most 8192 keys: within the default limit
-    evict_select_kernel<kSelectThreads><<<grid, kSelectThreads, key_cap * 4, s>>>(a, key_cap);
+  int ctas = 1;
+  while (a.max_context_len > kClusterTokens && ctas < kMostClusterCtas && 2 * ctas * pairs <= 148) ctas *= 2;
+  int key_cap = (a.max_context_len + ctas - 1) / ctas;
+  const int most = pairs <= 148 ? kMostKeys : kKeys;
+  if (key_cap > most) key_cap = most;
+  const int smem = key_cap * (int)sizeof(uint32_t);
+  const dim3 grid((unsigned)(a.num_kv_heads * ctas), (unsigned)a.num_seqs);
+  static std::atomic<uint64_t> one_done{0}, cluster_done{0};
+  if (ctas > 1) {
+    auto kern = evict_select_kernel<kSelectMostThreads, true>;
+    if (!ensure_smem_attr(kern, kMostKeys * 4, cluster_done)) return VASR_PA_ELAUNCH;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(kSelectMostThreads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {(unsigned)ctas, 1, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, kern, a, key_cap) != cudaSuccess) return VASR_PA_ELAUNCH;
+  } else if (pairs <= 148) {
+    auto kern = evict_select_kernel<kSelectMostThreads, false>;
+    if (!ensure_smem_attr(kern, kMostKeys * 4, one_done)) return VASR_PA_ELAUNCH;
+    kern<<<grid, kSelectMostThreads, smem, s>>>(a, key_cap);
+  } else {  // at most kKeys keys: within the default limit
+    evict_select_kernel<kSelectThreads, false><<<grid, kSelectThreads, smem, s>>>(a, key_cap);
   }
   switch (a.elem_size) {
     case 1: return launch_move<uint8_t>(a, s);

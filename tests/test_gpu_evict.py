@@ -100,6 +100,20 @@ def test_long_sequences(cuda_device, in_place):
     check(cuda_device, torch.bfloat16, (70001,), 1, 64, 32, 3001, 1, 64, "ties", in_place, seed=6)
 
 
+@pytest.mark.parametrize("kind", ["plain", "ties", "equal"])
+@pytest.mark.parametrize("seqs,hkv", [(4, 1), (4, 8), (4, 15), (4, 25), (5, 40)])
+def test_long_and_short_together(cuda_device, seqs, hkv, kind):
+    """Few and many (sequence, head)s share one long context's selection differently; the call's
+    bound, not a sequence's own length, decides."""
+    lens = (9001, 5, 0, 8193, 17)[:seqs]
+    check(cuda_device, FP8, lens, hkv, 16, 16, 600, 3, 100, kind, True, seed=20, bound=9001)
+
+
+def test_longer_than_the_keys_kept_at_hand(cuda_device):
+    check(cuda_device, FP8, (50001,), 80, 16, 32, 900, 2, 64, "ties", True, seed=21)
+    check(cuda_device, FP8, (400001,), 1, 16, 32, 900, 2, 64, "ties", False, seed=22)
+
+
 def test_twice_in_place(cuda_device):
     """A second eviction works on what the first one left (the other sequences' pages untouched)."""
     dev, bs, hkv, d = cuda_device, 16, 2, 64
