@@ -458,12 +458,15 @@ int32_t vasr_pa_greedy_argmax(uint32_t *next_ids, const void *logits,
  * axis the same positions) indexes cos_table / sin_table, f32
  * [max_position, R / 2]; a position outside is clamped and sets
  * VASR_PA_DERR_POSITION_RANGE. Dims R .. head_dim pass unrotated. sections is
- * a HOST array; num_axes is 1 to 4.
+ * a HOST array; num_axes is 1 to 4, R at most 512 (VASR_PA_ENOT_SUPPORTED).
+ * R = head_dim of 64, 128 or 256 with 16-byte aligned rows and tables runs
+ * fastest.
  *
  * mrope: x [num_tokens, num_heads, head_dim] with the given token and head
  * strides (elements; unit dim stride) -> out, strides likewise; out may be x.
  * inverse != 0 turns by the negative angle, which is also the gradient of the
- * forward rotation. f32, bf16 or f16; arithmetic in f32, one rounding.
+ * forward rotation. Rows of out must not overlap each other. f32, bf16 or f16;
+ * arithmetic in f32, one rounding.
  */
 int32_t vasr_pa_mrope(void *out, int64_t out_token_stride, int64_t out_head_stride, const void *x,
                       int64_t x_token_stride, int64_t x_head_stride, const float *cos_table,
@@ -508,8 +511,12 @@ int32_t vasr_pa_fused_qk_norm_mrope_append(
  * added in a fixed order. Block tables of different sequences must not name
  * the same block (it would be scored by both at once), except for the null
  * block that padding rows share, whose scores mean nothing. f32, bf16 or f16
- * queries over pages of the same type or fp8; the workspace is scratch that
- * needs no clearing, one call at a time.
+ * queries over pages of the same type or fp8; head_dim up to 512, query_len up
+ * to 64 (VASR_PA_ENOT_SUPPORTED), any number of query heads per kv head;
+ * head_dim 128 with up to 128 rows per kv head runs fastest. score_cache is
+ * 16-byte aligned. The workspace (256-byte aligned) is scratch that needs no
+ * clearing, one call at a time; it grows with max_context_len, which should
+ * be near the longest context.
  */
 size_t vasr_pa_paged_attention_scored_workspace_size(int32_t num_seqs, int32_t query_len,
                                                      int32_t score_rows, int32_t num_heads,
@@ -567,7 +574,7 @@ int32_t vasr_pa_evict_kv(void *key_cache, void *value_cache, float *score_cache,
  * Lowest index on ties; NaN logits count as -inf; a row without a logit above
  * -inf accepts nothing and gives token 0. draft_lens (may be NULL) shortens a
  * sequence's drafts; draft ids outside the vocabulary are rejected. num_drafts
- * 0 samples one token. out_tokens [num_seqs, num_drafts + 1]: the accepted
+ * (at most 1023) 0 samples one token. out_tokens [num_seqs, num_drafts + 1]: the accepted
  * drafts, the next token, then -1; num_accepted [num_seqs]. uniform and race
  * may be NULL when temperatures is NULL and temperature <= 0. workspace:
  * zeroed once before first use and left zeroed where it has to be; one call

@@ -10,6 +10,13 @@
 // The inverse turns by the negative angle; as the rotation is orthogonal it is
 // also the gradient of the forward form. All arithmetic is f32 and each output
 // is rounded once, when it is stored.
+//
+// Calls of a few tokens are bound by the latency of a launch and three
+// dependent loads (position, angle, store): 64 tokens of 16 + 8 + 8 heads of
+// 128 take 4.1 us. Long ones are bound by memory: 8192 such tokens (139 MB in
+// bf16, prompts into pages) take 29 us, 4.7 TB/s; 4099 tokens of 24 heads
+// turned back (52 MB) 12 us, 4.3 TB/s, much of it the start and end of the
+// launch. The general kernels below, a warp a row, took 157 and 35 us there.
 #include <type_traits>
 
 #include "common.cuh"
@@ -139,7 +146,9 @@ __global__ void __launch_bounds__(32 * kWarps) mrope_rows_kernel(const MropeArgs
 // Rows whose D / 2 rotated pairs fall into whole 16-byte chunks: a thread owns
 // chunk c and its partner c + C / 2 of a token's row (C chunks a row), so both
 // halves of its pairs are its own and the norm is a sum over the C / 2 lanes
-// of the row. It loads its cos and sin once and runs over the heads with them.
+// of the row. It loads its cos and sin once and runs over the heads with them
+// (a warp a row loads them again for every head). Every other R, head_dim,
+// stride or alignment takes the general kernels.
 template <int kX>
 struct Angles {
   float c[kX], s[kX];
@@ -226,6 +235,9 @@ constexpr int tile_warps(bool prompt) {
 // Prompts: the part's heads of the tile's rows arrive by one bulk copy a token
 // (a token's heads are adjacent), so that the bytes in flight cost shared
 // memory and not registers; rows are 16 bytes apart modulo 128 to spread banks.
+// Smaller parts mean more CTAs per SM and less imbalance at the end, until the
+// angles are loaded too often: 29 us at 8192 tokens, against 32 with parts of
+// 2048 bytes, 30 with 1536 and 31 with 1024.
 constexpr int kPartBytes = 1280;  // of one token's row at most
 template <typename T, int D>
 constexpr int part_heads() { return kPartBytes / (D * (int)sizeof(T)) > 0 ? kPartBytes / (D * (int)sizeof(T)) : 1; }
@@ -233,9 +245,10 @@ template <typename T, int D>
 constexpr int part_pitch() { return part_heads<T, D>() * D * (int)sizeof(T) + 16; }
 
 // grid = (token tile, part): the first qk_parts parts share the tile's q and k
-// heads, the others its V. Warps split a tile's tokens and its heads. V goes out element by element with the tile's tokens across the
-// lanes: consecutive slots fill a page row's 32-byte sectors whole in one
-// store, and any other slots need no case of their own.
+// heads, the others its V. Warps split a tile's tokens and its heads. V goes
+// out element by element with the tile's tokens across the lanes: consecutive
+// slots fill a page row's 32-byte sectors whole in one store, and any other
+// slots need no case of their own.
 template <typename T, typename TC, int D, bool kPrompt>
 __global__ void __launch_bounds__(32 * tile_warps<T, D>(kPrompt)) mrope_append_tile_kernel(const MropeAppendArgs p,
                                                                                           int qk_parts) {
@@ -429,6 +442,8 @@ bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0;
 // Calls of kPromptTokens or more take the prompt form: 5.1 against 5.4 us at
 // 512 tokens (16 + 8 heads of 128), 5.6 / 7.0 at 1000, 4.5 / 4.0 at 256.
 constexpr int kPromptTokens = 512;
+// Short calls split the heads over more CTAs until there are this many: 12.1 us
+// at 4099 tokens of 24 heads, against 15.3 with half and 13.3 with twice as many.
 constexpr int kTargetCtas = 4 * 148;
 
 template <typename T, typename TC, int D, bool kPrompt>
