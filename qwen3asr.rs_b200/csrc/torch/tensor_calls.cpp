@@ -12,14 +12,17 @@
 #include <Python.h>
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <initializer_list>
 #include <map>
 #include <string>
 #include <utility>
+#include <vector>
 
 #include "vasr_pa.h"
 
@@ -142,23 +145,29 @@ void check(int status, const char *what) {
 }
 
 // One growing, zero-filled workspace per (device, stream) for one kind of call.
+// It is allocated and filled on that stream, whichever is current. Outgrown
+// ones stay allocated, since captured graphs may hold their addresses; growing
+// by doubling bounds them by the one in use.
 class Workspaces {
  public:
   explicit Workspaces(const char *what) : what_(what) {}
   const at::Tensor &reserve(c10::DeviceIndex device, uintptr_t stream, size_t bytes) {
-    at::Tensor &ws = held_[{device, stream}];
-    if (!ws.defined() || (size_t)ws.numel() < bytes) {
+    std::vector<at::Tensor> &all = held_[{device, stream}];
+    const size_t have = all.empty() ? 0 : (size_t)all.back().numel();
+    if (all.empty() || have < bytes) {
       if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
         throw Refused{VASR_PA_EINVAL_WORKSPACE, what_ + " workspace must be reserved before CUDA graph capture"};
-      ws = at::zeros({(int64_t)(bytes < (1u << 20) ? (1u << 20) : bytes)},
-                     at::TensorOptions().dtype(at::kByte).device(c10::Device(c10::kCUDA, device)));
+      const c10::cuda::CUDAStreamGuard guard(
+          c10::cuda::getStreamFromExternal(reinterpret_cast<cudaStream_t>(stream), device));
+      all.push_back(at::zeros({(int64_t)std::max({bytes, 2 * have, (size_t)1 << 20})},
+                              at::TensorOptions().dtype(at::kByte).device(c10::Device(c10::kCUDA, device))));
     }
-    return ws;
+    return all.back();
   }
 
  private:
   std::string what_;
-  std::map<std::pair<c10::DeviceIndex, uintptr_t>, at::Tensor> held_;
+  std::map<std::pair<c10::DeviceIndex, uintptr_t>, std::vector<at::Tensor>> held_;
 };
 Workspaces &scored_workspaces() {
   static auto *w = new Workspaces("paged_attention_scored");  // outlives the interpreter's tensors
@@ -214,6 +223,7 @@ PyObject *mrope(PyObject *const *a) {
   const bool interleaved = truth(a[5]), inverse = truth(a[6]);
   const at::Tensor *given = maybe(a[7], "out");
   const c10::DeviceIndex dev = common_device({&x, &cos, &sin, &pos});
+  const c10::cuda::CUDAGuard on_device(dev);
   require(x.dim() == 3 && x.stride(2) == 1, VASR_PA_EINVAL_SHAPE, "x must be [T, H, D] with unit dim stride");
   const int64_t t = x.size(0), h = x.size(1), d = x.size(2);
   const Rope r = rope_of(cos, sin, pos, a[4], t);
@@ -240,6 +250,7 @@ PyObject *mrope_append(PyObject *const *a) {
   const at::Tensor *ks = maybe(a[13], "k_scale"), *vs = maybe(a[14], "v_scale"), *scores = maybe(a[15], "score_cache"),
                    *given = maybe(a[16], "q_out");
   const c10::DeviceIndex dev = common_device({&qkv, &kc, &vc, &pos, &slots, &cos, &sin});
+  const c10::cuda::CUDAGuard on_device(dev);
   const Cache c = cache_of(kc, vc);
   require(hq > 0 && qkv.dim() == 2 && qkv.stride(1) == 1 && qkv.size(1) == ((int64_t)hq + 2 * c.heads) * c.dim,
           VASR_PA_EINVAL_SHAPE, "qkv must be [T, (Hq + 2 Hkv) * D] with unit column stride");
@@ -285,6 +296,7 @@ PyObject *scored(PyObject *const *a) {
   const float scale = (float)real(a[9]), softcap = (float)real(a[10]), decay = (float)real(a[11]);
   const at::Tensor *given = maybe(a[13], "out");
   const c10::DeviceIndex dev = common_device({&q, &kc, &vc, &scores, &bt, &cl});
+  const c10::cuda::CUDAGuard on_device(dev);
   const Cache c = cache_of(kc, vc);
   const int64_t dims = q.dim();
   require(dims == 3 || dims == 4, VASR_PA_EINVAL_SHAPE, "q must be [B, Hq, D] or [B, W, Hq, D] with packed heads");
@@ -332,6 +344,7 @@ PyObject *evict(PyObject *const *a) {
                 sink = whole32(a[7], "num_sink"), recent = whole32(a[8], "num_recent");
   const at::Tensor *lim = maybe(a[9], "budgets"), *to = maybe(a[10], "out_block_tables");
   const c10::DeviceIndex dev = common_device({&kc, &vc, &scores, &bt, &cl});
+  const c10::cuda::CUDAGuard on_device(dev);
   const Cache c = cache_of(kc, vc);
   check_scores(scores, c, dev);
   require(bt.dim() == 2, VASR_PA_EINVAL_SHAPE, "block_tables must be u32/i32 [B, cols]");
@@ -365,6 +378,7 @@ PyObject *verify(PyObject *const *a) {
   const at::Tensor *probs = maybe(a[2], "draft_probs"), *uni = maybe(a[3], "uniform"), *race = maybe(a[4], "race"),
                    *len = maybe(a[6], "draft_lens");
   const c10::DeviceIndex dev = common_device({&logits, &dt});
+  const c10::cuda::CUDAGuard on_device(dev);
   require(logits.dim() == 3 && logits.stride(2) == 1 && logits.size(1) >= 1, VASR_PA_EINVAL_SHAPE,
           "target_logits must be [B, K + 1, V] with unit column stride");
   const int64_t b = logits.size(0), k = logits.size(1) - 1, v = logits.size(2);

@@ -249,3 +249,32 @@ def test_loose_bound_leaves_the_order_of_the_stream(cuda_device):
         assert torch.equal(out, got[0][0]) and torch.equal(s, got[0][1])
     # the 16 query heads' weights of every sequence sum to 16
     assert abs(float(got[-1][1].double().sum()) - 64 * 16) < 64 * 16 * 1e-4
+
+
+def test_a_captured_graph_outlives_a_larger_call(cuda_device):
+    """The workspace grows for the larger call; the graph still works in the one it was captured with."""
+    dev = cuda_device
+    q, kc, vc, old, bt, ctx = check(dev, torch.bfloat16, torch.bfloat16, (900, 513, 64), 4, 2, 128, 16, seed=31)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        need = eviction.paged_attention_scored_workspace_bytes(3, 1, 1, 4, 2, 128, 16, 900)
+        small = eviction.reserve_paged_attention_scored_workspace(dev, need)
+        s = old.clone()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            out = eviction.paged_attention_scored(q[:, 0], None, None, kc, vc, s, bt, ctx, 900, 0.1)
+        s.copy_(old)
+        g.replay()
+        want, want_s = out.clone(), s.clone()
+        large = eviction.reserve_paged_attention_scored_workspace(dev, 2 * small.numel())
+        assert large.data_ptr() != small.data_ptr() and large.numel() >= 2 * small.numel()
+        at, size = small.data_ptr(), small.numel()
+        del small
+        taken = [torch.full((size,), 255, dtype=torch.uint8, device=dev) for _ in range(4)]
+        assert all(t.data_ptr() + size <= at or at + size <= t.data_ptr() for t in taken)  # still held
+        s.copy_(old)
+        g.replay()
+        assert torch.equal(out, want) and torch.equal(s, want_s)
+        assert all(bool((t == 255).all()) for t in taken)
+    torch.cuda.synchronize()

@@ -181,3 +181,26 @@ def test_stream_and_graph(cuda_device):
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     del g
+
+
+def test_workspace_of_another_stream_is_filled_on_it(cuda_device):
+    """Reserving for a stream that is not current zeroes the workspace in that stream's order."""
+    dev = cuda_device
+    rng = np.random.default_rng(41)
+    logits, drafts, _, uniform, race = inputs(rng, 3, 2, 50000, torch.float32, None)
+    ins = [torch.as_tensor(x).to(dev) for x in (logits, drafts, uniform, race)]
+    want = speculative.verify_draft_tokens(ins[0], ins[1], None, ins[2], ins[3], 1.0)
+    stream = torch.cuda.Stream()
+    need = speculative.verify_draft_tokens_workspace_bytes(3, 2, 50000)
+    torch.cuda.synchronize()
+    torch.cuda._sleep(20_000_000)  # the current stream is busy: a fill on it would come after the call
+    speculative.reserve_verify_draft_tokens_workspace(dev, need, stream)
+    with torch.cuda.stream(stream):
+        got = speculative.verify_draft_tokens(ins[0], ins[1], None, ins[2], ins[3], 1.0)
+    stream.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        again = speculative.verify_draft_tokens(ins[0], ins[1], None, ins[2], ins[3], 1.0)
+    stream.synchronize()
+    assert torch.equal(again[0], want[0])
