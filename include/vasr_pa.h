@@ -515,8 +515,9 @@ int32_t vasr_pa_fused_qk_norm_mrope_append(
  * to 64 (VASR_PA_ENOT_SUPPORTED), any number of query heads per kv head;
  * head_dim 128 with up to 128 rows per kv head runs fastest. score_cache is
  * 16-byte aligned. The workspace (256-byte aligned) is scratch that needs no
- * clearing, one call at a time; it grows with max_context_len, which should
- * be near the longest context.
+ * clearing, one call at a time; it is sized for the call's own arguments (a
+ * smaller call may split its contexts further) and grows with
+ * max_context_len, which should be near the longest context.
  */
 size_t vasr_pa_paged_attention_scored_workspace_size(int32_t num_seqs, int32_t query_len,
                                                      int32_t score_rows, int32_t num_heads,

@@ -40,7 +40,7 @@ bool takes_split(const ScoredArgs &a) {
          (int64_t)a.num_kv_heads * ((rows + 1) / 2) <= 65535;
 }
 
-constexpr int kSplitMostTokens = 1024;
+constexpr int kSplitMostTokens = 1024, kSplitFewTokens = 640, kSplitFewPairs = 4 * 148;
 
 struct SplitLayout {
   int pages_per_split, max_splits;
@@ -52,15 +52,22 @@ SplitLayout split_layout(int num_seqs, int query_len, int score_rows, int num_he
   SplitLayout l;
   // Splits of 1024 tokens, or shorter ones that just fill the SMs once (three
   // CTAs each) where the longest contexts would leave some idle; at least 64.
-  // 512 sequences of 64 to 4096 tokens: 324 us with 1024, 325 with 768, 333
-  // with 512, 393 with 256 (more partial results to join). One of 16381: 17.9
-  // us with three CTAs a SM, 21.1 with four, of which the last wait for places.
+  // 512 sequences of 64 to 4096 tokens, 8 kv heads: 324 us with 1024, 325 with
+  // 768, 333 with 512, 393 with 256 (more partial results to join). One of
+  // 16381: 17.9 us with three CTAs a SM, 21.1 with four, of which the last wait
+  // for places. Few (sequence, kv head)s of up to two splits end at different
+  // times: 640 tokens took 48 against 52 us for 64 windows of 5 rows over 200
+  // to 1500 tokens, 29.7 / 33.1 for 32, 39.5 / 40.7 for 64 single tokens, 76 /
+  // 79 in f32, 31.3 / 31.1 from fp8 pages; but 82.6 / 78.7 for 128 windows, 192
+  // / 186 for 64 windows over 4000 tokens.
   const int64_t pairs = (int64_t)num_seqs * num_kv_heads;
   const int pages = (max_context_len + block_size - 1) / block_size;
   int64_t per_pair = 3 * 148 / pairs;
   if (per_pair < 1) per_pair = 1;
   int64_t want = (pages + per_pair - 1) / per_pair;
-  const int least = (64 + block_size - 1) / block_size, most = kSplitMostTokens / block_size;
+  const int least = (64 + block_size - 1) / block_size;
+  const bool few = pairs <= kSplitFewPairs && max_context_len <= 2 * kSplitMostTokens;
+  const int most = (few ? kSplitFewTokens : kSplitMostTokens) / block_size;
   l.pages_per_split = (int)(want < least ? least : want > most ? most : want);
   if (l.pages_per_split > kScoredMaxPages) l.pages_per_split = kScoredMaxPages;
   const int per = l.pages_per_split * block_size;

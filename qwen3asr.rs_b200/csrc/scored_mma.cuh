@@ -31,8 +31,8 @@
 // tokens (68 MB) takes 18 us (3.8 TB/s; the split alone 13.4). fp8 pages and
 // windows are bound by instructions and by how evenly the contexts fall on the
 // SMs: 64 sequences of 200 to 1500 tokens take 31 us from fp8 pages (99 MB;
-// SMs busy 68% of the time, the schedulers issue in 42% of the cycles) and 53
-// us for windows of 5 f16 rows (197 MB; 74%, 33%).
+// SMs busy 68% of the time, the schedulers issue in 42% of the cycles) and 48
+// us for windows of 5 f16 rows (197 MB).
 #pragma once
 
 #include "decode_mma.cuh"
