@@ -13,13 +13,15 @@
 // a last one that lists the survivors by rank. A CTA has a (sequence, kv head);
 // long contexts of few sequences take a cluster of CTAs, which add their
 // histograms up over distributed shared memory. It is bound by latency: 8
-// heads of 4099 tokens take about 10 us of launch, loads and barriers.
+// heads of 4099 tokens take about 8 us of launch, loads and barriers. Plain
+// shared atomics count fastest, equal scores included: one count per distinct
+// digit of a warp, found by a match, took 2 us more.
 //
 // The move copies bits, bound by memory: it reads every 32-byte sector that
 // holds a kept token and writes the kept ones. A sector of V holds 16 tokens
 // of one dim (16-bit pages), so that nearly all of V is read whatever stays:
 // 640 of 700 to 1500 tokens of 64 sequences are 342 MB of kept K, V and scores,
-// 428 MB of sectors, and take 94 us with the selection (the move alone 81% of
+// 428 MB of sectors, and take 92 us with the selection (the move alone 81% of
 // the copy rate in sectors). In place, token r of the result comes from an
 // index >= r, so places filled in ascending tiles never overwrite a token that
 // is still needed, as long as a tile is read before it or a later one is
@@ -39,7 +41,7 @@ namespace vasr {
 namespace {
 
 constexpr int kSelectThreads = 512;
-constexpr int kSelectMostThreads = 1024;  // at most 148 (sequence, head)s: 16 against 18 us for 8 of 4099 tokens
+constexpr int kSelectMostThreads = 1024;  // at most 148 (sequence, head)s: measured 16 against 18 us for 8 of 4099 tokens
 // Keys in a CTA's shared memory: 32 KB, or most of an SM's where every CTA has
 // one to itself (one sequence of 32768 tokens, one CTA a head: 62 against 96 us).
 constexpr int kKeys = 8192, kMostKeys = 49152;
@@ -135,10 +137,7 @@ __global__ void __launch_bounds__(kThreads) evict_select_kernel(const EvictArgs 
       const int j = j0 + tid;
       const uint32_t key = j < t1 ? key_of(j) : 0u;
       const bool in = j < t1 && (key & mask) == prefix;
-      // one count per distinct digit of the warp: scores share their leading bytes
-      const uint32_t digit = in ? (key >> shift8) & 255u : 256u;
-      const uint32_t same = __match_any_sync(0xffffffffu, digit);
-      if (in && lane == __ffs(same) - 1) atomicAdd(&hist[digit], __popc(same));
+      if (in) atomicAdd(&hist[(key >> shift8) & 255u], 1);
     }
     if constexpr (kCluster) {
       cluster.sync();
