@@ -204,10 +204,8 @@ __global__ void __launch_bounds__(kThreads) evict_select_kernel(const EvictArgs 
     ties = __reduce_add_sync(0xffffffffu, lower_cta.y);
     cluster.barrier_arrive();  // this CTA has read the others' shared memory
   }
-  for (int w = 0; w < warp; ++w) {
-    above += s_above[w];
-    ties += s_ties[w];
-  }
+  above += __reduce_add_sync(0xffffffffu, lane < warp ? s_above[lane] : 0);
+  ties += __reduce_add_sync(0xffffffffu, lane < warp ? s_ties[lane] : 0);
   const uint32_t lower = (1u << lane) - 1u;
   for (int j = j0; j < j1; j += 32) {
     const int mine = j + lane;
