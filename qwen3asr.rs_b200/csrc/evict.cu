@@ -41,13 +41,14 @@ namespace vasr {
 namespace {
 
 constexpr int kSelectThreads = 512;
-constexpr int kSelectMostThreads = 1024;  // at most 148 (sequence, head)s: measured 16 against 18 us for 8 of 4099 tokens
+constexpr int kSelectMostThreads = 1024;  // at most 148 (sequence, head)s: 13.8 against 15.3 us for 8 of 4099 tokens
 // Keys in a CTA's shared memory: 32 KB, or most of an SM's where every CTA has
-// one to itself (one sequence of 32768 tokens, one CTA a head: 62 against 96 us).
+// one to itself (one CTA a head of 20000 tokens: 43 against 57 us for 8 heads, 85
+// / 101 for 32).
 constexpr int kKeys = 8192, kMostKeys = 49152;
 // Longer contexts of up to 74 (sequence, head)s take clusters of up to 8 CTAs:
-// 21 against 26 us at 8 heads of 9000 tokens, 30 / 51 at 20000, 79 / 92 at 32
-// heads of 20000; at 2000 tokens 14.5 / 11.6, at 32 heads of 4099 24 / 22.6.
+// 20.5 against 22.5 us at 8 heads of 9000 tokens, 29 / 43 at 20000, 75 / 85 at 32
+// heads of 20000; but 15.3 / 13.8 at 8 of 4099, 23 / 20 at 32 of 4099.
 constexpr int kClusterTokens = 8192, kMostClusterCtas = 8;
 constexpr int kMoveThreads = 256;
 constexpr int kMoveMostThreads = 1024;
@@ -305,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == kMoveThreads ? 4 : 1) ev
 
 // CTAs per (sequence, head): enough to fill the SMs, at most one per unit.
 // Where even that leaves most SMs' places empty, tiles of 1024 tokens take fewer
-// turns: 15.9 against 17.3 us at one sequence of 4099 tokens, 62 / 70 at 32768.
+// turns: 13.8 against 15.2 us at one sequence of 4099 tokens, 29 / 42 at 20000.
 template <typename U, int BS>
 int launch_move_bs(const EvictArgs &a, cudaStream_t s) {
   const int chunks = a.head_dim * (int)sizeof(U) / 16;
