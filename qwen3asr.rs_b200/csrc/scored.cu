@@ -16,7 +16,8 @@
 // scored_f32_kernel (f32 queries and pages, scored_f32.cuh); the kernels here
 // serve the other shapes, one thread a token, three launches (121 us for one
 // sequence of 16381 tokens, 2410 us for 512 of 64 to 4096, which the others
-// take 18 and 324 us for).
+// take 17 and 317 us for). Comparisons below that name 324 us were made
+// while the join's registers spilled, which cost 7 us on both sides.
 #include "common.cuh"
 #include "launch.h"
 #include "scored_f32.cuh"

@@ -25,12 +25,12 @@
 // as in decode_mma.cuh, so that one ldmatrix row of 16 bytes feeds a k-step.
 //
 // With bf16 pages and one token a sequence this is bound by memory: 512
-// sequences of 64 to 4096 tokens, 16 heads over 8, are 2.00 GB and take 324 us
-// with the join (6.2 TB/s; 291 us without any scores). mma.sync suffices: at 2
+// sequences of 64 to 4096 tokens, 16 heads over 8, are 2.00 GB and take 317 us
+// with the join (6.3 TB/s; 291 us without any scores). mma.sync suffices: at 2
 // to 10 rows a 128-row tcgen05 tile would be empty. One sequence of 16381
-// tokens (68 MB) takes 18 us (3.8 TB/s; the split alone 13.4). fp8 pages and
+// tokens (68 MB) takes 17 us (3.9 TB/s; the split alone 13.4). fp8 pages and
 // windows are bound by instructions and by how evenly the contexts fall on the
-// SMs: 64 sequences of 200 to 1500 tokens take 31 us from fp8 pages (99 MB;
+// SMs: 64 sequences of 200 to 1500 tokens take 30 us from fp8 pages (99 MB;
 // SMs busy 68% of the time, the schedulers issue in 42% of the cycles) and 48
 // us for windows of 5 f16 rows (197 MB).
 #pragma once
