@@ -25,13 +25,13 @@
 // twice, the second time from L2.
 //
 // A large call is bound by memory and, nearly as much, by the exponentials: 64
-// sequences of 5 bf16 rows of 151936 logits with an f32 drafter take 47 us for
-// the 175 MB that must be read (3.7 TB/s), 32 x 8 f32 rows without a drafter
-// 40 us (4.4 TB/s). One sequence takes 8.9 us, the latency of three launches
+// sequences of 5 bf16 rows of 151936 logits with an f32 drafter take 43 us for
+// the 175 MB that must be read (4.1 TB/s), 32 x 8 f32 rows without a drafter
+// 40 us (4.4 TB/s). One sequence takes 9.1 us, the latency of three launches
 // that each wait for one round of loads; CTAs of 64 threads, four times as
-// many, took 11.7 us there (more chunks to join) and 52 us for the large call.
+// many, took 11.7 us there (more chunks to join) and 5 us more for the large call.
 // CTAs that stay and load the next chunk ahead of the current one's work need
-// registers for two, and were slower (50 us).
+// registers for two, and were slower by 3 us.
 #include <type_traits>
 
 #include "common.cuh"
@@ -43,6 +43,13 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kRowElems = 32;   // logits a thread of the first launch keeps (16: 49 us for the large call)
 constexpr int kEmitElems = 16;  // of logits, drafter's values and noise each, in the third (8: 59 us, 32: 48 us)
+// CTAs a SM whose registers suffice: at 64 x 5 bf16 rows 42.7 us with 8 and 5,
+// 46.0 with 6 and 4, 47.6 with 8 and 6; at 32 x 8 f32 rows, which hold twice the
+// registers, 39.8 with 5, 41.6 with 4, 47.4 with 6.
+template <typename T>
+constexpr int kRowCtas = sizeof(T) == 2 ? 8 : 5;
+template <typename T>
+constexpr int kEmitCtas = sizeof(T) == 2 ? 5 : 4;
 
 // One chunk of a row: its maximum (and, for greedy rows, the first place of
 // it) and sum over the chunk of exp((x - max) / T).
@@ -181,7 +188,7 @@ __device__ __forceinline__ void each_of_group(const Held<T, kGroups> &x, int k, 
 
 // grid = (chunk, row, sequence)
 template <typename T>
-__global__ void __launch_bounds__(kThreads) verify_rows_kernel(const VerifyArgs p) {
+__global__ void __launch_bounds__(kThreads, kRowCtas<T>) verify_rows_kernel(const VerifyArgs p) {
   pdl_launch_dependents();
   constexpr int kGroups = kRowElems / kGroup;
   __shared__ float2 part[kThreads / 32];
@@ -325,7 +332,7 @@ __global__ void __launch_bounds__(kThreads) verify_verdict_kernel(const VerifyAr
 
 // grid = (chunk, sequence)
 template <typename T, typename TQ>
-__global__ void __launch_bounds__(kThreads, 4) verify_emit_kernel(const VerifyArgs p) {
+__global__ void __launch_bounds__(kThreads, kEmitCtas<T>) verify_emit_kernel(const VerifyArgs p) {
   constexpr int kGroups = kEmitElems / kGroup;
   __shared__ Best part[kThreads / 32];
   const int chunk = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
