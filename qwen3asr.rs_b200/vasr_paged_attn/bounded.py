@@ -23,6 +23,8 @@ from . import _lib, eviction, fused, speculative
 from . import mistralrs_paged_attn as pa
 from .engine import RandomQwen3Decoder, allocate_paged_cache
 
+MAX_WINDOW = 64  # rows a sequence that paged_attention_scored takes
+
 
 def lookup_drafts(tokens: Sequence[int], count: int) -> list[int]:
     """Drafts read off the sequence itself: what followed the last earlier occurrence of its last
@@ -99,6 +101,8 @@ class BoundedSpeculativeDecoder:
         """Shrinks every sequence to the budget once one of them has no place for ``rows`` more."""
         if longest + rows <= self.capacity:
             return
+        if min(longest, self.budget) + rows > self.capacity:  # the slots would lie past the block table
+            raise _lib.VasrPaError(_lib.EINVAL_SHAPE, f"no room for {rows} tokens beside a budget of {self.budget}")
         lens = self.context_lens
         for (kc, vc), scores in zip(self.caches, self.scores):
             _, lens = eviction.evict_kv(kc, vc, scores, self.block_tables, self.context_lens, self.capacity,
@@ -107,19 +111,27 @@ class BoundedSpeculativeDecoder:
         self.evictions += 1
 
     def prefill(self, prompts: Sequence[Sequence[int]], window: int = 16) -> None:
-        """Prompts of one length, ``window`` tokens at a time; all but the last token, which the
-        first step's window begins with. Every row of a prompt's windows scores the cache."""
+        """Prompts of one length, ``window`` tokens at a time (fewer where an eviction leaves room for
+        fewer, and at most the attention's 64); all but the last token, which the first step's window
+        begins with. Every row of a prompt's windows scores the cache."""
         length = len(prompts[0])
         if length < 1 or any(len(p) != length for p in prompts) or len(prompts) != self.num_seqs:
             raise _lib.VasrPaError(_lib.EINVAL_SHAPE, "prompts must be num_seqs sequences of one length")
+        if window < 1:
+            raise _lib.VasrPaError(_lib.EINVAL_SHAPE, "window must be at least one token")
         self.tokens = [list(p) for p in prompts]
         ids = torch.tensor(self.tokens, device=self.device)
-        for at in range(0, length - 1, window):
-            rows = min(window, length - 1 - at)
-            self._make_room(rows, int(self.context_lens.max()))
+        at = 0
+        while at < length - 1:
+            longest = int(self.context_lens.max())
+            rows = min(window, MAX_WINDOW, length - 1 - at)
+            if longest + rows > self.capacity:
+                rows = min(rows, self.capacity - min(longest, self.budget))
+            self._make_room(rows, longest)
             self._layers(ids[:, at:at + rows], rows, None)
             self.context_lens = self.context_lens + rows
             self.next_positions += rows
+            at += rows
 
     def step(self) -> list[list[int]]:
         """The tokens that this step adds to each sequence: the accepted drafts and one more."""
