@@ -69,6 +69,7 @@ class BoundedSpeculativeDecoder:
         self.next_positions = torch.zeros(num_seqs, dtype=torch.int64, device=dev)
         self.tokens: list[list[int]] = [[] for _ in range(num_seqs)]
         self.evictions = 0
+        self.max_positions = model.rope_cos.shape[0]
         self._gen = torch.Generator(device=dev).manual_seed(seed)
 
     def _layers(self, ids: torch.Tensor, rows: int, score_rows: Optional[int]) -> torch.Tensor:
@@ -119,6 +120,8 @@ class BoundedSpeculativeDecoder:
             raise _lib.VasrPaError(_lib.EINVAL_SHAPE, "prompts must be num_seqs sequences of one length")
         if window < 1:
             raise _lib.VasrPaError(_lib.EINVAL_SHAPE, "window must be at least one token")
+        if length - 1 > self.max_positions:
+            raise _lib.VasrPaError(_lib.EINVAL_SHAPE, f"a prompt of {length} tokens leaves the rotary tables")
         self.tokens = [list(p) for p in prompts]
         ids = torch.tensor(self.tokens, device=self.device)
         at = 0
@@ -134,8 +137,15 @@ class BoundedSpeculativeDecoder:
             at += rows
 
     def step(self) -> list[list[int]]:
-        """The tokens that this step adds to each sequence: the accepted drafts and one more."""
-        b, k, dev = self.num_seqs, self.num_drafts, self.device
+        """The tokens that this step adds to each sequence: the accepted drafts and one more.
+
+        Positions run on while the cache is shrunk: near the end of the rotary tables a step drafts
+        less, and one past it is refused."""
+        b, dev = self.num_seqs, self.device
+        at = max(len(t) for t in self.tokens) - 1  # the window's first position
+        if at >= self.max_positions:
+            raise _lib.VasrPaError(_lib.EINVAL_SHAPE, f"position {at} leaves the rotary tables")
+        k = min(self.num_drafts, self.max_positions - 1 - at)
         drafts = torch.tensor([lookup_drafts(t, k) for t in self.tokens], dtype=torch.int32, device=dev).view(b, k)
         last = torch.tensor([t[-1] for t in self.tokens], device=dev)
         self._make_room(k + 1, int(self.context_lens.max()))

@@ -94,3 +94,33 @@ def test_a_window_that_cannot_fit_is_refused_on_the_host(stubs):
     assert e.value.status == _lib.EINVAL_SHAPE
     with pytest.raises(_lib.VasrPaError):
         dec.prefill(prompts(30), 0)
+
+
+def test_positions_stay_within_the_rotary_tables(stubs):
+    """The cache is bounded, positions are not: a prompt that needs rows past the tables is refused,
+    drafts are given up near their end, and a step past it is refused."""
+    dec = decoder(4, 64, 40, max_positions=50)
+    with pytest.raises(_lib.VasrPaError) as e:
+        dec.prefill(prompts(51 + 1))
+    assert e.value.status == _lib.EINVAL_SHAPE and not stubs.positions
+    dec.prefill(prompts(44))
+    for _ in range(7):  # first rows at 43 .. 49
+        assert all(len(new) == 1 for new in dec.step())
+    assert [len(w) // 2 for w in stubs.positions[-7:]] == [5, 5, 5, 4, 3, 2, 1]
+    lens, tokens = dec.context_lens.tolist(), [list(t) for t in dec.tokens]
+    with pytest.raises(_lib.VasrPaError) as e:
+        dec.step()
+    assert e.value.status == _lib.EINVAL_SHAPE
+    assert dec.context_lens.tolist() == lens and dec.tokens == tokens
+
+
+def test_the_longest_sequence_limits_the_drafts(stubs):
+    dec = decoder(4, 64, 40, max_positions=50)
+    dec.prefill(prompts(40))
+    dec.tokens[1] += [1] * 6
+    dec.next_positions[1] += 6
+    dec.step()
+    assert stubs.positions[-1] == list(range(39, 44)) + list(range(45, 50))
+    stubs.accept = 4
+    dec.step()
+    assert stubs.positions[-1][-1] <= 49
