@@ -4,9 +4,9 @@ One step per call, for a batch of sequences: the last emitted token and K drafte
 the decoder as a window of K + 1 rows (``fused.qk_norm_mrope_append`` appends them and clears their
 scores, ``eviction.paged_attention_scored`` attends and scores the cache with the window's first
 row, the only one known to stay), ``speculative.verify_draft_tokens`` keeps a prefix of the drafts
-and draws the next token, and a sequence whose pages run full is shrunk to its budget by
-``eviction.evict_kv``, layer by layer and kv head by kv head. Positions run on while the cache
-shrinks, so a token's position is no longer its place in the cache.
+and draws the next token, and once a sequence's pages run full every sequence longer than the budget
+is shrunk to it by ``eviction.evict_kv``, layer by layer and kv head by kv head. Positions run on
+while the cache shrinks, so a token's position is no longer its place in the cache.
 
 The reference decodes one greedy token a step over a cache that only grows
 (vasr-models/src/model/paged_batch_engine.rs:609-730); with temperature 0 and a budget that is
@@ -122,6 +122,10 @@ class BoundedSpeculativeDecoder:
             raise _lib.VasrPaError(_lib.EINVAL_SHAPE, "window must be at least one token")
         if length - 1 > self.max_positions:
             raise _lib.VasrPaError(_lib.EINVAL_SHAPE, f"a prompt of {length} tokens leaves the rotary tables")
+        # a decoder that has decoded before starts afresh: the appends clear the slots' old scores
+        self.context_lens = torch.zeros_like(self.context_lens)
+        self.next_positions = torch.zeros_like(self.next_positions)
+        self.evictions = 0
         self.tokens = [list(p) for p in prompts]
         ids = torch.tensor(self.tokens, device=self.device)
         at = 0

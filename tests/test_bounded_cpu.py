@@ -124,3 +124,16 @@ def test_the_longest_sequence_limits_the_drafts(stubs):
     stubs.accept = 4
     dec.step()
     assert stubs.positions[-1][-1] <= 49
+
+
+def test_a_second_prompt_starts_afresh(stubs):
+    dec = decoder(3, 64, 40)
+    dec.prefill(prompts(100))
+    for _ in range(10):
+        dec.step()
+    assert dec.evictions > 0
+    del stubs.positions[:]
+    dec.prefill(prompts(20))
+    assert dec.context_lens.tolist() == [19, 19] and dec.next_positions.tolist() == [19, 19]
+    assert dec.evictions == 0 and dec.tokens == prompts(20)
+    assert [p[:16] for p in stubs.positions] == [list(range(16)), [16, 17, 18, 16, 17, 18]]
