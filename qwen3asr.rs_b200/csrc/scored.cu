@@ -119,6 +119,7 @@ __device__ __forceinline__ int context_of(const ScoredArgs &a, int b) {
   }
   return (int)n;
 }
+// The page to read for token j: block 0 stands in for one that is none of the pool's.
 __device__ __forceinline__ int64_t page_of(const ScoredArgs &a, int b, int j) {
   const uint32_t id = a.block_tables[(int64_t)b * a.max_num_blocks_per_seq + j / a.block_size];
   if ((int64_t)id < a.num_blocks) return id;
@@ -236,6 +237,8 @@ __global__ void __launch_bounds__(kWeightThreads) scored_weight_kernel(const Sco
   const int n = context_of(a, b);
   const int j = blockIdx.x * kWeightThreads + threadIdx.x;
   if (j >= n) return;
+  const uint32_t id = a.block_tables[(int64_t)b * a.max_num_blocks_per_seq + j / a.block_size];
+  if ((int64_t)id >= a.num_blocks) return;  // no page of the pool's (recorded where it was read): no score
   float sum = 0.f;
   for (int i = 0; i < a.score_rows; ++i)
     for (int g = 0; g < p.group; ++g) {
@@ -244,7 +247,7 @@ __global__ void __launch_bounds__(kWeightThreads) scored_weight_kernel(const Sco
       const float x = p.x[(((int64_t)b * a.score_rows + i) * a.num_heads + head) * p.x_stride + j];
       if (ml.y != 0.f) sum += exp2f(x - ml.x) / ml.y;
     }
-  float *s = a.score_cache + (page_of(a, b, j) * a.num_kv_heads + kvh) * a.block_size + j % a.block_size;
+  float *s = a.score_cache + ((int64_t)id * a.num_kv_heads + kvh) * a.block_size + j % a.block_size;
   *s = a.decay * *s + sum;
 }
 
