@@ -342,8 +342,10 @@ constexpr int ring_stages() {
 
 template <typename T, typename TC, int BS, int NRT, bool kDup>
 int launch_mma_rows(const ScoredArgs &a, cudaStream_t s) {
-  // one-byte pages leave room for four CTAs a SM: 31 against 34 us for 64 sequences of 200 to 1500 tokens
-  constexpr int kNST = ring_stages<TC, BS>(), kMinB = sizeof(TC) == 1 && NRT == 1 ? 4 : 3;
+  // one-byte pages leave room for four CTAs a SM: 31 against 34 us for 64
+  // sequences of 200 to 1500 tokens; but windows, whose P comes in two
+  // products, would spill there (windows of 4 rows 42.8 against 38.9 us)
+  constexpr int kNST = ring_stages<TC, BS>(), kMinB = sizeof(TC) == 1 && kDup ? 4 : 3;
   static std::atomic<uint64_t> attr_done{0};
   return launch_split<T, ScoredCfg<TC, BS, kNST>, BS>(a, scored_mma_kernel<T, TC, BS, NRT, kDup, kNST, kMinB>, attr_done,
                                                       kDup ? 4 : 8 * NRT, s);
@@ -367,12 +369,10 @@ int launch_f32_bs(const ScoredArgs &a, cudaStream_t s) {
 template <typename T, typename TC, int BS>
 int launch_mma_bs(const ScoredArgs &a, cudaStream_t s) {
   const int rows = a.query_len * (a.num_heads / a.num_kv_heads);
-  // bf16 over fp8 pages: P is rounded to f16, 8 times finer than the output; doubled rows would gain nothing
-  constexpr bool kDup = !(std::is_same<T, __nv_bfloat16>::value && sizeof(TC) == 1);
   // Doubled rows cost nothing in time (18.3 / 17.9 us without / with them for
   // one sequence) and are taken wherever they fit. Tiles of 16 rows for 8 rows
   // would: 50 against 44 us for 64 sequences' windows of 4 rows.
-  if (rows <= 4 && kDup) return launch_mma_rows<T, TC, BS, 1, kDup>(a, s);
+  if (rows <= 4) return launch_mma_rows<T, TC, BS, 1, true>(a, s);
   if (rows <= 8) return launch_mma_rows<T, TC, BS, 1, false>(a, s);
   return launch_mma_rows<T, TC, BS, 2, false>(a, s);
 }

@@ -7,12 +7,17 @@
 //   S[16 rows x 16] = Q K^T     A = Q, B = K by ldmatrix from the page layout
 //   O^T[128 x rows] += V^T P^T  A = V^T by ldmatrix, B = S's own fragments
 //
-// Up to 4 rows (kDup: one token, group <= 4) P^T has columns to spare: A holds
-// every query row twice, so the score fragments of rows r and r + 4 are equal,
-// and row r's P goes into the product rounded to the operand type while row
-// r + 4 carries what that rounding left. O then has P's full f32 precision up
-// to 2^-16, for no further MMA; with more rows P is rounded to the operand
-// type (the output has that rounding anyway).
+// P enters its product in two parts of the operand type, what it rounds to and
+// what that rounding left, so that O has P to 2^-16 (bf16) or 2^-22 (f16) and a
+// window's rows answer as single tokens do. Up to 4 rows (kDup: one token,
+// group <= 4) P^T has columns to spare: A holds every query row twice, so the
+// score fragments of rows r and r + 4 are equal, and row r + 4 carries row r's
+// rest for no further MMA. With more rows the rest takes MMAs of its own. P
+// rounded alone was 2.8 instead of 2.1 parts in 10^4 off 64 bits for windows of
+// 5 f16 rows (2.1 is the output's own rounding) and took, in us through the
+// public call, 50.7 against 52.9 there, 43.9 / 45.1 for windows of 4 bf16 rows,
+// 326 / 348 for 256 windows of 5 over 500 to 4000 tokens, 121 / 129 for 16 rows
+// all scored, 37.6 / 38.9 for windows of 4 over fp8 pages.
 //
 // Tokens that only some rows of a window see (the last query_len - 1) stay
 // out of the P V product: a masked row would multiply their V by zero, and a
@@ -176,7 +181,7 @@ __global__ void __launch_bounds__(kScoredThreads, MINB) scored_mma_kernel(const 
       auto tok = [&](int nn, int e) { return kFp8 ? t0 + 4 * tig + 2 * nn + e : t0 + nn * 8 + tig * 2 + e; };
       const bool tail = t0 + 16 > whole;
       float pv[NRT][4];
-      uint32_t pa[NRT][2];
+      uint32_t pa[NRT][2], rest[NRT][2];  // P in the operand type, and what that rounding left
 #pragma unroll
       for (int t = 0; t < NRT; ++t) {
         float x[4];
@@ -224,12 +229,9 @@ __global__ void __launch_bounds__(kScoredThreads, MINB) scored_mma_kernel(const 
 #pragma unroll
         for (int nn = 0; nn < 2; ++nn) {
           pa[t][nn] = dec_pack2<TM>(pv[t][2 * nn], pv[t][2 * nn + 1]);
-          if constexpr (kDup) {  // rows 4..7: what the rounding of rows 0..3 left
-            const TM *h = reinterpret_cast<const TM *>(&pa[t][nn]);
-            const uint32_t rest = dec_pack2<TM>(pv[t][2 * nn] - Elem<TM>::to_f32(h[0]),
-                                                pv[t][2 * nn + 1] - Elem<TM>::to_f32(h[1]));
-            if (grp >= 4) pa[t][nn] = rest;
-          }
+          const TM *h = reinterpret_cast<const TM *>(&pa[t][nn]);
+          rest[t][nn] = dec_pack2<TM>(pv[t][2 * nn] - Elem<TM>::to_f32(h[0]), pv[t][2 * nn + 1] - Elem<TM>::to_f32(h[1]));
+          if (kDup && grp >= 4) pa[t][nn] = rest[t][nn];  // rows 4..7: the rest of rows 0..3
         }
       }
       // ---- O^T += V^T P^T over the tokens that every row sees
@@ -254,7 +256,10 @@ __global__ void __launch_bounds__(kScoredThreads, MINB) scored_mma_kernel(const 
               a3 &= mhi;
             }
 #pragma unroll
-            for (int t = 0; t < NRT; ++t) dec_mma<TM>(o[t][dq * 2 + hf], a0, a1, a2, a3, pa[t][0], pa[t][1]);
+            for (int t = 0; t < NRT; ++t) {
+              dec_mma<TM>(o[t][dq * 2 + hf], a0, a1, a2, a3, pa[t][0], pa[t][1]);
+              if constexpr (!kDup) dec_mma<TM>(o[t][dq * 2 + hf], a0, a1, a2, a3, rest[t][0], rest[t][1]);
+            }
           }
         }
       } else {
@@ -275,7 +280,10 @@ __global__ void __launch_bounds__(kScoredThreads, MINB) scored_mma_kernel(const 
             b3 &= m1;
           }
 #pragma unroll
-          for (int t = 0; t < NRT; ++t) dec_mma<TM>(o[t][dp], b0, b2, b1, b3, pa[t][0], pa[t][1]);
+          for (int t = 0; t < NRT; ++t) {
+            dec_mma<TM>(o[t][dp], b0, b2, b1, b3, pa[t][0], pa[t][1]);
+            if constexpr (!kDup) dec_mma<TM>(o[t][dp], b0, b2, b1, b3, rest[t][0], rest[t][1]);
+          }
         }
       }
       // ---- tokens that only some rows see, one by one
