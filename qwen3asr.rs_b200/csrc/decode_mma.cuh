@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(128, MINB) paged_decode_mma_kernel(const Decod
     const int n_valid = min(C::kST, tok_end - (tok_begin + u * C::kST));
     const uint32_t sk = s_base + C::kOffK + s * C::kSP * C::kPB;
     const uint32_t sv = s_base + C::kOffV + s * C::kSP * C::kPB;
-    dec_mma_stage<T, BS, D, TC, C::kNTT, C::kPB, kQSmem>(sk, sv, n_valid, qa, s_q, c_log2, use_softcap, p.scale,
+    dec_mma_stage<T, BS, D, TC, C::kNTT, C::kPB, kQSmem>(sk, sv, n_valid, qa, s_q, c_log2, use_softcap, k_mul,
                                                   p.softcap, o, m_used, l_part);
     __syncwarp();
     const int nu = u + C::kNST;
