@@ -8,6 +8,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <mutex>
 
 #include "launch.h"
 
@@ -797,23 +798,36 @@ int32_t vasr_pa_verify_draft_tokens(
   return vasr::launch_verify(a, to_stream(stream));
 }
 
+namespace {
+// The units' error words, ORed into one (and cleared) by a single launch.
+struct ErrorWords {
+  uint32_t *word[9];
+};
+__device__ uint32_t g_error_bits;
+__global__ void collect_errors_kernel(const ErrorWords w, bool clear) {
+  uint32_t bits = 0;
+  for (uint32_t *word : w.word) bits |= clear ? atomicExch(word, 0u) : atomicOr(word, 0u);
+  g_error_bits = bits;
+}
+}  // namespace
+
 int32_t vasr_pa_get_device_error(int32_t *out_bits, int32_t clear, vasr_pa_stream_t stream) {
   if (!out_bits) return VASR_PA_EINVAL_POINTER;
-  uint32_t a = 0, b = 0, c = 0, d = 0, e = 0;
-  int r;
-  if ((r = vasr::read_error_kv_ops(&a, clear != 0, to_stream(stream))) != VASR_PA_OK) return r;
-  if ((r = vasr::read_error_decode(&b, clear != 0, to_stream(stream))) != VASR_PA_OK) return r;
-  if ((r = vasr::read_error_prefill(&c, clear != 0, to_stream(stream))) != VASR_PA_OK) return r;
-  if ((r = vasr::read_error_fused(&d, clear != 0, to_stream(stream))) != VASR_PA_OK) return r;
-  if ((r = vasr::read_error_prefill_umma(&e, clear != 0, to_stream(stream))) != VASR_PA_OK)
-    return r;
-  uint32_t f = 0;
-  if ((r = vasr::read_error_decode_loop(&f, clear != 0, to_stream(stream))) != VASR_PA_OK) return r;
-  uint32_t g = 0, h = 0, i = 0;
-  if ((r = vasr::read_error_mrope(&g, clear != 0, to_stream(stream))) != VASR_PA_OK) return r;
-  if ((r = vasr::read_error_scored(&h, clear != 0, to_stream(stream))) != VASR_PA_OK) return r;
-  if ((r = vasr::read_error_evict(&i, clear != 0, to_stream(stream))) != VASR_PA_OK) return r;
-  *out_bits = (int32_t)(a | b | c | d | e | f | g | h | i);
+  const ErrorWords w{{vasr::error_word_kv_ops(), vasr::error_word_decode(), vasr::error_word_prefill(),
+                      vasr::error_word_fused(), vasr::error_word_prefill_umma(), vasr::error_word_decode_loop(),
+                      vasr::error_word_mrope(), vasr::error_word_scored(), vasr::error_word_evict()}};
+  for (const uint32_t *word : w.word)
+    if (!word) return VASR_PA_ELAUNCH;
+  static std::mutex one_reader;  // of g_error_bits
+  const std::lock_guard<std::mutex> lock(one_reader);
+  const cudaStream_t s = to_stream(stream);
+  uint32_t bits = 0;
+  collect_errors_kernel<<<1, 1, 0, s>>>(w, clear != 0);
+  if (cudaPeekAtLastError() != cudaSuccess ||
+      cudaMemcpyFromSymbolAsync(&bits, g_error_bits, sizeof(bits), 0, cudaMemcpyDeviceToHost, s) != cudaSuccess ||
+      cudaStreamSynchronize(s) != cudaSuccess)
+    return VASR_PA_ELAUNCH;
+  *out_bits = (int32_t)bits;
   return VASR_PA_OK;
 }
 

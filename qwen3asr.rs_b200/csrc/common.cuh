@@ -24,19 +24,10 @@ __device__ __forceinline__ void raise_device_error(uint32_t bits) {
   atomicOr(&g_device_error, bits);
 }
 
-// Read (and optionally clear) this unit's error word; synchronises the stream.
-static inline int read_unit_error(uint32_t *bits, bool clear, cudaStream_t s) {
-  uint32_t v = 0;
-  const uint32_t zero = 0;
-  if (cudaMemcpyFromSymbolAsync(&v, g_device_error, sizeof(v), 0, cudaMemcpyDeviceToHost, s) != cudaSuccess ||
-      cudaStreamSynchronize(s) != cudaSuccess)
-    return VASR_PA_ELAUNCH;
-  if (clear && (cudaMemcpyToSymbolAsync(g_device_error, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, s) !=
-                    cudaSuccess ||
-                cudaStreamSynchronize(s) != cudaSuccess))
-    return VASR_PA_ELAUNCH;
-  *bits = v;
-  return VASR_PA_OK;
+// Address of this unit's error word on the current device (null: no device).
+static inline uint32_t *unit_error_word() {
+  void *word = nullptr;
+  return cudaGetSymbolAddress(&word, g_device_error) == cudaSuccess ? static_cast<uint32_t *>(word) : nullptr;
 }
 
 // ---------------------------------------------------------------- elements

@@ -379,6 +379,6 @@ int launch_evict(const EvictArgs &a, cudaStream_t s) {
   }
 }
 
-int read_error_evict(uint32_t *bits, bool clear, cudaStream_t s) { return read_unit_error(bits, clear, s); }
+uint32_t *error_word_evict() { return unit_error_word(); }
 
 }  // namespace vasr

@@ -1469,21 +1469,6 @@ int launch_swap_blocks(void *dst, const void *src, const int64_t *mapping, int64
   return cudaPeekAtLastError() == cudaSuccess ? VASR_PA_OK : VASR_PA_ELAUNCH;
 }
 
-int read_error_kv_ops(uint32_t *bits, bool clear, cudaStream_t s) {
-  uint32_t v = 0;
-  if (cudaMemcpyFromSymbolAsync(&v, g_device_error, sizeof(v), 0, cudaMemcpyDeviceToHost, s) !=
-      cudaSuccess)
-    return VASR_PA_ELAUNCH;
-  if (cudaStreamSynchronize(s) != cudaSuccess) return VASR_PA_ELAUNCH;
-  if (clear) {
-    const uint32_t z = 0;
-    if (cudaMemcpyToSymbolAsync(g_device_error, &z, sizeof(z), 0, cudaMemcpyHostToDevice, s) !=
-        cudaSuccess)
-      return VASR_PA_ELAUNCH;
-    if (cudaStreamSynchronize(s) != cudaSuccess) return VASR_PA_ELAUNCH;
-  }
-  *bits = v;
-  return VASR_PA_OK;
-}
+uint32_t *error_word_kv_ops() { return unit_error_word(); }
 
 }  // namespace vasr

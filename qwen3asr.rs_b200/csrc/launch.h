@@ -181,7 +181,7 @@ struct MropeArgs {
   int dtype;
 };
 int launch_mrope(const MropeArgs &a, cudaStream_t s);
-int read_error_mrope(uint32_t *bits, bool clear, cudaStream_t s);
+uint32_t *error_word_mrope();
 
 // Decode attention over a window of query_len rows a sequence that adds every
 // visible token's weight to its score (scored.cu).
@@ -217,7 +217,7 @@ struct ScoredArgs {
 size_t scored_workspace_bytes(int num_seqs, int query_len, int score_rows, int num_heads,
                               int num_kv_heads, int head_dim, int block_size, int max_context_len);
 int launch_scored(const ScoredArgs &a, cudaStream_t s);
-int read_error_scored(uint32_t *bits, bool clear, cudaStream_t s);
+uint32_t *error_word_scored();
 
 // Selection of the tokens that stay in the cache and their move to the front
 // of the sequence's pages (evict.cu).
@@ -245,7 +245,7 @@ struct EvictArgs {
   int elem_size;
 };
 int launch_evict(const EvictArgs &a, cudaStream_t s);
-int read_error_evict(uint32_t *bits, bool clear, cudaStream_t s);
+uint32_t *error_word_evict();
 
 // Acceptance of drafted tokens and the token that follows (verify.cu).
 struct VerifyArgs {
@@ -319,8 +319,8 @@ struct ArgmaxArgs {
 void argmax_chunking(int64_t vocab, int *num_chunks, int64_t *chunk_elems);
 size_t argmax_workspace_bytes(int num_seqs, int64_t vocab);
 int launch_greedy_argmax(ArgmaxArgs a, void *workspace, cudaStream_t s);
-int read_error_decode_loop(uint32_t *bits, bool clear, cudaStream_t s);
-int read_error_fused(uint32_t *bits, bool clear, cudaStream_t s);
+uint32_t *error_word_decode_loop();
+uint32_t *error_word_fused();
 
 // Workspace layout of the decode kernel (all offsets 256-byte aligned):
 // [counters: kDecodeMaxCounters x u32][partial o][partial (m, l)].
@@ -375,10 +375,10 @@ int launch_swap_blocks(void *dst, const void *src, const int64_t *mapping, int64
                        int64_t src_blocks, int64_t dst_blocks, int64_t block_bytes,
                        cudaStream_t s);
 
-int read_error_kv_ops(uint32_t *bits, bool clear, cudaStream_t s);
-int read_error_decode(uint32_t *bits, bool clear, cudaStream_t s);
-int read_error_prefill(uint32_t *bits, bool clear, cudaStream_t s);
-int read_error_prefill_umma(uint32_t *bits, bool clear, cudaStream_t s);
+uint32_t *error_word_kv_ops();
+uint32_t *error_word_decode();
+uint32_t *error_word_prefill();
+uint32_t *error_word_prefill_umma();
 
 // Raise a kernel's dynamic shared-memory limit once per device. The
 // attribute is not a stream operation, so this is legal during capture.

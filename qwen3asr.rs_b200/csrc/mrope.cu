@@ -551,8 +551,6 @@ int launch_mrope(const MropeArgs &a, cudaStream_t s) {
   }
 }
 
-int read_error_mrope(uint32_t *bits, bool clear, cudaStream_t s) {
-  return read_unit_error(bits, clear, s);
-}
+uint32_t *error_word_mrope() { return unit_error_word(); }
 
 }  // namespace vasr

@@ -1066,21 +1066,6 @@ int launch_prefill_umma(const PrefillArgs &a, cudaStream_t s) {
   }
 }
 
-int read_error_prefill_umma(uint32_t *bits, bool clear, cudaStream_t s) {
-  uint32_t v = 0;
-  if (cudaMemcpyFromSymbolAsync(&v, g_device_error, sizeof(v), 0, cudaMemcpyDeviceToHost, s) !=
-      cudaSuccess)
-    return VASR_PA_ELAUNCH;
-  if (cudaStreamSynchronize(s) != cudaSuccess) return VASR_PA_ELAUNCH;
-  if (clear) {
-    const uint32_t z = 0;
-    if (cudaMemcpyToSymbolAsync(g_device_error, &z, sizeof(z), 0, cudaMemcpyHostToDevice, s) !=
-        cudaSuccess)
-      return VASR_PA_ELAUNCH;
-    if (cudaStreamSynchronize(s) != cudaSuccess) return VASR_PA_ELAUNCH;
-  }
-  *bits = v;
-  return VASR_PA_OK;
-}
+uint32_t *error_word_prefill_umma() { return unit_error_word(); }
 
 }  // namespace vasr

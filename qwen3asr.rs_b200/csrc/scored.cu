@@ -423,6 +423,6 @@ int launch_scored(const ScoredArgs &a, cudaStream_t s) {
   }
 }
 
-int read_error_scored(uint32_t *bits, bool clear, cudaStream_t s) { return read_unit_error(bits, clear, s); }
+uint32_t *error_word_scored() { return unit_error_word(); }
 
 }  // namespace vasr
