@@ -577,9 +577,8 @@ int32_t vasr_pa_evict_kv(void *key_cache, void *value_cache, float *score_cache,
  * sequence's drafts; draft ids outside the vocabulary are rejected. num_drafts
  * (at most 1023) 0 samples one token. out_tokens [num_seqs, num_drafts + 1]: the accepted
  * drafts, the next token, then -1; num_accepted [num_seqs]. uniform and race
- * may be NULL when temperatures is NULL and temperature <= 0. workspace:
- * zeroed once before first use and left zeroed where it has to be; one call
- * at a time per workspace.
+ * may be NULL when temperatures is NULL and temperature <= 0. workspace
+ * (256-byte aligned) is scratch that needs no clearing, one call at a time.
  */
 size_t vasr_pa_verify_draft_tokens_workspace_size(int32_t num_seqs, int32_t num_drafts,
                                                   int64_t vocab);

@@ -144,10 +144,15 @@ void check(int status, const char *what) {
   if (status != VASR_PA_OK) throw Refused{status, what};
 }
 
-// One growing, zero-filled workspace per (device, stream) for one kind of call.
-// It is allocated and filled on that stream, whichever is current. Outgrown
-// ones stay allocated, since captured graphs may hold their addresses; growing
-// by doubling bounds them by the one in use.
+bool capturing() {
+  return c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None;
+}
+
+// The scratch of one kind of call: a growing workspace per (device, stream),
+// allocated in that stream's order, whichever is current; outgrown ones stay
+// allocated, and doubling bounds them by the one in use. A call that is being
+// captured takes its scratch from the graph's own memory instead: graphs that
+// were captured on one stream may be replayed on several at once.
 class Workspaces {
  public:
   explicit Workspaces(const char *what) : what_(what) {}
@@ -155,17 +160,23 @@ class Workspaces {
     std::vector<at::Tensor> &all = held_[{device, stream}];
     const size_t have = all.empty() ? 0 : (size_t)all.back().numel();
     if (all.empty() || have < bytes) {
-      if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
-        throw Refused{VASR_PA_EINVAL_WORKSPACE, what_ + " workspace must be reserved before CUDA graph capture"};
+      if (capturing())
+        throw Refused{VASR_PA_EINVAL_WORKSPACE, what_ + " workspace cannot be reserved while a CUDA graph is captured"};
       const c10::cuda::CUDAStreamGuard guard(
           c10::cuda::getStreamFromExternal(reinterpret_cast<cudaStream_t>(stream), device));
-      all.push_back(at::zeros({(int64_t)std::max({bytes, 2 * have, (size_t)1 << 20})},
-                              at::TensorOptions().dtype(at::kByte).device(c10::Device(c10::kCUDA, device))));
+      all.push_back(allocate(device, std::max({bytes, 2 * have, (size_t)1 << 20})));
     }
     return all.back();
   }
+  at::Tensor scratch(c10::DeviceIndex device, vasr_pa_stream_t stream, size_t bytes) {
+    if (capturing()) return allocate(device, std::max(bytes, (size_t)1));
+    return reserve(device, reinterpret_cast<uintptr_t>(stream), bytes);
+  }
 
  private:
+  static at::Tensor allocate(c10::DeviceIndex device, size_t bytes) {
+    return at::empty({(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(c10::Device(c10::kCUDA, device)));
+  }
   std::string what_;
   std::map<std::pair<c10::DeviceIndex, uintptr_t>, std::vector<at::Tensor>> held_;
 };
@@ -319,7 +330,7 @@ PyObject *scored(PyObject *const *a) {
   const at::Tensor out = given ? *given : at::empty(q.sizes(), q.options());
   const vasr_pa_stream_t stream = stream_of(dev);
   const size_t need = c_scored_size((int32_t)b, (int32_t)window, rows, (int32_t)hq, c.heads, c.dim, c.block, longest);
-  const at::Tensor &ws = scored_workspaces().reserve(dev, reinterpret_cast<uintptr_t>(stream), need);
+  const at::Tensor ws = scored_workspaces().scratch(dev, stream, need);
   check(c_scored(ptr(out), ptr(q), ptr(kc), ptr(vc), ptr<float>(scores), ptr<uint32_t>(tables), ptr<uint32_t>(lens),
                  (int32_t)b, (int32_t)window, rows, (int32_t)hq, c.heads, c.dim, c.block, c.blocks, (int32_t)tables.size(1),
                  longest, scale, softcap, decay, q_stride, code, c.code, c.fp8 ? ptr<float>(ks) : nullptr,
@@ -408,8 +419,7 @@ PyObject *verify(PyObject *const *a) {
   const at::Tensor uniform = uni ? uni->contiguous() : at::Tensor(), lens = len ? len->contiguous() : at::Tensor();
   const at::Tensor tokens = at::empty({b, k + 1}, dt.options()), accepted = at::empty({b}, dt.options());
   const vasr_pa_stream_t stream = stream_of(dev);
-  const at::Tensor &ws = verify_workspaces().reserve(dev, reinterpret_cast<uintptr_t>(stream),
-                                                     c_verify_size((int32_t)b, (int32_t)k, v));
+  const at::Tensor ws = verify_workspaces().scratch(dev, stream, c_verify_size((int32_t)b, (int32_t)k, v));
   check(c_verify(ptr<int32_t>(tokens), ptr<int32_t>(accepted), ptr(logits), logits.stride(0), logits.stride(1), code,
                  ptr<int32_t>(drafts), len ? ptr<int32_t>(lens) : nullptr, ptr(probs), probs ? probs->stride(0) : 0,
                  probs ? probs->stride(1) : 0, probs ? dtype_code(*probs) : 0, uni ? ptr<float>(uniform) : nullptr,
@@ -420,7 +430,7 @@ PyObject *verify(PyObject *const *a) {
 }
 
 // ------------------------------------------------------------------- workspaces
-// reserve(kind, device index, stream handle, bytes) -> the workspace
+// reserve(kind, device index, stream handle, bytes) -> the stream's workspace
 PyObject *reserve(PyObject *const *a) {
   const int64_t kind = whole(a[0]);
   Workspaces &w = kind == 0 ? scored_workspaces() : verify_workspaces();

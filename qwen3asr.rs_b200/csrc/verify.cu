@@ -21,7 +21,8 @@
 // launch wait for its own atomic (40 against 30 us at 64 x 5 rows of 151936).
 // The third runs the race over row n, a CTA per chunk of the vocabulary: it
 // has its noise in registers by the time the verdict is there, and the last
-// CTA of a sequence takes the winner. Only the row that is drawn from is read
+// CTA of a sequence takes the winner, found by a counter that the second launch
+// has zeroed (so the workspace needs no clearing). Only the row that is drawn from is read
 // twice, the second time from L2.
 //
 // A large call is bound by memory and, nearly as much, by the exponentials: 64
@@ -323,6 +324,7 @@ __global__ void __launch_bounds__(kThreads) verify_verdict_kernel(const VerifyAr
   const bool drawn = t > 0.f && s.max > -INFINITY;
   if (tid == 0) {
     static_cast<Verdict *>(p.verdicts)[b] = Verdict{n, s.max, 1.f / s.sum, drawn};
+    p.counters[b] = 0u;  // of the race's CTAs
     p.num_accepted[b] = n;
   }
   int32_t *out = p.out_tokens + (int64_t)b * (p.num_drafts + 1);  // all but the drawn token
@@ -431,17 +433,15 @@ __global__ void __launch_bounds__(kThreads, kEmitCtas<T>) verify_emit_kernel(con
     }
     best = warp_best(best);
   }
-  if (lane == 0) {
+  if (lane == 0)
     p.out_tokens[(int64_t)b * (p.num_drafts + 1) + s.n] = best.i != kNone ? (int32_t)best.i : 0;  // 0: all noise NaN
-    p.counters[b] = 0u;
-  }
 }
 
 struct VerifyLayout {
   int row_chunks, emit_chunks;
   size_t off_stats, off_verdicts, off_bests, total;
 };
-constexpr size_t kCounterBytes = 65536 * sizeof(uint32_t);  // one per sequence, left at zero
+constexpr size_t kCounterBytes = 65536 * sizeof(uint32_t);  // one per sequence, zeroed by the second launch
 VerifyLayout verify_layout(int num_seqs, int num_drafts, int64_t vocab) {
   VerifyLayout l;
   auto chunks = [&](int elems) { return (int)((vocab + kThreads * elems - 1) / (kThreads * elems)); };

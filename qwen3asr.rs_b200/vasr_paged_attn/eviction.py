@@ -32,7 +32,9 @@ def paged_attention_scored_workspace_bytes(num_seqs: int, query_len: int, score_
 
 def reserve_paged_attention_scored_workspace(device: torch.device, nbytes: int,
                                              stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
-    """Make sure the stream's scratch holds ``nbytes``; call before a CUDA-graph capture."""
+    """Make sure the stream's scratch holds ``nbytes``, so that calls on it do not have to grow it.
+
+    Calls that a CUDA graph captures take theirs from the graph's own memory."""
     return _calls.reserve(_calls.SCORED, device, nbytes, stream)
 
 

@@ -21,7 +21,9 @@ def verify_draft_tokens_workspace_bytes(num_seqs: int, num_drafts: int, vocab: i
 
 def reserve_verify_draft_tokens_workspace(device: torch.device, nbytes: int,
                                           stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
-    """Make sure the stream's workspace holds ``nbytes``; call before a CUDA-graph capture."""
+    """Make sure the stream's workspace holds ``nbytes``, so that calls on it do not have to grow it.
+
+    Calls that a CUDA graph captures take theirs from the graph's own memory."""
     return _calls.reserve(_calls.VERIFY, device, nbytes, stream)
 
 
