@@ -345,9 +345,9 @@ int launch_evict(const EvictArgs &a, cudaStream_t s) {
   const int64_t pairs = (int64_t)a.num_seqs * a.num_kv_heads;
   int ctas = 1;
   while (a.max_context_len > kClusterTokens && ctas < kMostClusterCtas && 2 * ctas * pairs <= 148) ctas *= 2;
-  int key_cap = (a.max_context_len + ctas - 1) / ctas;
+  const int64_t share = ((int64_t)a.max_context_len + ctas - 1) / ctas;
   const int most = pairs <= 148 ? kMostKeys : kKeys;
-  if (key_cap > most) key_cap = most;
+  const int key_cap = share > most ? most : (int)share;
   const int smem = key_cap * (int)sizeof(uint32_t);
   const dim3 grid((unsigned)(a.num_kv_heads * ctas), (unsigned)a.num_seqs);
   static std::atomic<uint64_t> one_done{0}, cluster_done{0};

@@ -62,7 +62,7 @@ SplitLayout split_layout(int num_seqs, int query_len, int score_rows, int num_he
   // 79 in f32, 31.3 / 31.1 from fp8 pages; but 82.6 / 78.7 for 128 windows, 192
   // / 186 for 64 windows over 4000 tokens.
   const int64_t pairs = (int64_t)num_seqs * num_kv_heads;
-  const int pages = (max_context_len + block_size - 1) / block_size;
+  const int64_t pages = ((int64_t)max_context_len + block_size - 1) / block_size;
   int64_t per_pair = 3 * 148 / pairs;
   if (per_pair < 1) per_pair = 1;
   int64_t want = (pages + per_pair - 1) / per_pair;
@@ -72,7 +72,7 @@ SplitLayout split_layout(int num_seqs, int query_len, int score_rows, int num_he
   l.pages_per_split = (int)(want < least ? least : want > most ? most : want);
   if (l.pages_per_split > kScoredMaxPages) l.pages_per_split = kScoredMaxPages;
   const int per = l.pages_per_split * block_size;
-  l.max_splits = (max_context_len + per - 1) / per;
+  l.max_splits = (int)(((int64_t)max_context_len + per - 1) / per);
   l.x_stride = (int64_t)l.max_splits * per;
   const size_t rows = (size_t)num_seqs * num_kv_heads * l.max_splits * query_len * (num_heads / num_kv_heads);
   l.off_o = 0;
@@ -90,7 +90,7 @@ struct ScoredLayout {
 };
 ScoredLayout layout(int num_seqs, int query_len, int score_rows, int num_heads, int head_dim, int max_context_len) {
   ScoredLayout l;
-  l.splits = (max_context_len + kSplitTokens - 1) / kSplitTokens;
+  l.splits = (int)(((int64_t)max_context_len + kSplitTokens - 1) / kSplitTokens);
   l.x_stride = (int64_t)l.splits * kSplitTokens;
   const size_t rows = (size_t)num_seqs * query_len * num_heads;
   l.off_o = 0;
@@ -263,7 +263,7 @@ int launch_scored_t(const ScoredArgs &a, cudaStream_t s) {
   scored_split_kernel<T, TC><<<dim3((unsigned)l.splits, (unsigned)a.num_heads, (unsigned)a.num_seqs), kThreads,
                                (a.head_dim + kSplitTokens) * sizeof(float), s>>>(p);
   scored_merge_kernel<T><<<(unsigned)rows, kMergeThreads, 0, s>>>(p);
-  const unsigned chunks = (unsigned)((a.max_context_len + kWeightThreads - 1) / kWeightThreads);
+  const unsigned chunks = ((unsigned)a.max_context_len + kWeightThreads - 1) / kWeightThreads;
   scored_weight_kernel<<<dim3(chunks, (unsigned)a.num_kv_heads, (unsigned)a.num_seqs), kWeightThreads, 0, s>>>(p);
   return cudaPeekAtLastError() == cudaSuccess ? VASR_PA_OK : VASR_PA_ELAUNCH;
 }
@@ -317,8 +317,9 @@ int launch_split(const ScoredArgs &a, void (*kern)(ScoredSplitParams), std::atom
   // warp each; at 4 splits the CTA is 326 against 324 us)
   const int64_t pairs = (int64_t)a.num_seqs * a.num_kv_heads;
   int chunk = 512;
-  while (chunk < a.max_context_len && pairs * ((a.max_context_len + chunk - 1) / chunk) > 16 * 148) chunk *= 2;
-  const int chunks = (a.max_context_len + chunk - 1) / chunk;
+  auto chunks_of = [&](int tokens) { return (int)(((int64_t)a.max_context_len + tokens - 1) / tokens); };
+  while (chunk < a.max_context_len && chunk < 1 << 30 && pairs * chunks_of(chunk) > 16 * 148) chunk *= 2;
+  const int chunks = chunks_of(chunk);
   const int row_warps = l.max_splits <= 8 ? 1 : kScoredThreads / 32;
   const int row_ctas = (p.rows * row_warps + kScoredThreads / 32 - 1) / (kScoredThreads / 32);
   cudaLaunchConfig_t cfg{};
