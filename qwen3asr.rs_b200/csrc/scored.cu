@@ -42,6 +42,7 @@ bool takes_split(const ScoredArgs &a) {
 }
 
 constexpr int kSplitMostTokens = 1024, kSplitFewTokens = 640, kSplitFewPairs = 4 * 148;
+static_assert(kSplitMostTokens <= kWeightTokens, "a context of one split has its scores added in one turn");
 
 struct SplitLayout {
   int pages_per_split, max_splits;

@@ -412,11 +412,7 @@ struct ScoredSplit {
         scored_out_row<T>(p, b, kvh, r)[d] = Elem<T>::from_f32(row_dim(r, d, f.x) * inv * v_mul);
       }
       __syncthreads();
-      weights.finish(p, fin, x, x_stride);
-      for (int j = kWeightTokens; j < n; j += kWeightTokens) {  // splits of pages of 32 tokens may be longer
-        weights.load(p, b, kvh, BS, j, n, x, x_stride);
-        weights.finish(p, fin, x, x_stride);
-      }
+      weights.finish(p, fin, x, x_stride);  // all of the context: a split is at most kWeightTokens long
       return;
     }
     for (int e = tid; e < rows_here * D; e += kScoredThreads) {
