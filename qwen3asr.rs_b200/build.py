@@ -7,7 +7,8 @@
   Rust API (metadata builders, block manager, graph buckets) as a pybind11
   module, used by the Python package and the tests.
 * ``lib/_vasr_calls*.so`` — the tensor-level entry points whose host cost counts
-  (g++ against torch's headers); the kernels stay in ``libvasr_pa.so``.
+  (g++ against torch's headers; left out where torch is not installed); the kernels stay in
+  ``libvasr_pa.so``.
 
 Objects go to ``_build/``; each unit is rebuilt only when it or a header it
 may include is newer than its object. Run ``python build.py`` or call
@@ -114,10 +115,15 @@ def build_host() -> Path | None:
     return out
 
 
-def build_calls() -> Path:
+def build_calls() -> Path | None:
     """Compile the torch extension module of ``csrc/torch`` (no link to the kernels: it is bound to
-    the loaded library at run time)."""
-    import torch  # noqa: PLC0415
+    the loaded library at run time). Without torch there is nothing to call it from: users of the C
+    ABI or the Rust shim alone get the library and the host module."""
+    try:
+        import torch  # noqa: PLC0415
+    except ImportError:
+        print("torch is not installed: the module _vasr_calls is not built", file=sys.stderr)
+        return None
 
     LIB.mkdir(exist_ok=True)
     out = LIB / f"_vasr_calls{sysconfig.get_config_var('EXT_SUFFIX') or '.so'}"
