@@ -71,6 +71,7 @@ def mrope(x: torch.Tensor, cos_table: torch.Tensor, sin_table: torch.Tensor, pos
     """Rotate x [T, H, D] by ``positions`` [axes, T] (see ``qk_norm_mrope_append``).
 
     ``inverse`` turns back; as the rotation is orthogonal that is also the gradient: with
-    y = mrope(x), dL/dx = mrope(dL/dy, inverse=True). ``out`` may be x; dims past 2 * sum(sections)
-    pass unchanged."""
+    y = mrope(x), dL/dx = mrope(dL/dy, inverse=True). Autograd does not record the call: the output
+    requires no gradient whatever x does, and a backward pass makes the inverse call itself. ``out``
+    may be x; dims past 2 * sum(sections) pass unchanged."""
     return calls().mrope(x, cos_table, sin_table, positions, sections, interleaved, inverse, out)
