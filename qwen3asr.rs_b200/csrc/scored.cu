@@ -58,10 +58,11 @@ SplitLayout split_layout(int num_seqs, int query_len, int score_rows, int num_he
   // 768, 333 with 512, 393 with 256 (more partial results to join). One of
   // 16381: 17.9 us with three CTAs a SM, 21.1 with four, of which the last wait
   // for places. Few (sequence, kv head)s of up to two splits end at different
-  // times: 640 tokens took 48 against 52 us for 64 windows of 5 rows over 200
-  // to 1500 tokens, 29.7 / 33.1 for 32, 39.5 / 40.7 for 64 single tokens, 76 /
-  // 79 in f32, 31.3 / 31.1 from fp8 pages; but 82.6 / 78.7 for 128 windows, 192
-  // / 186 for 64 windows over 4000 tokens.
+  // times: 640 tokens took 50.4 against 55.9 us for 64 windows of 5 rows over
+  // 200 to 1500 tokens, 29.9 / 36.1 for 32, 42.4 / 45.2 for 64 of 4 rows, 38.3 /
+  // 40.1 for 64 single tokens, 76 / 79 in f32, 30.9 / 30.8 from fp8 pages; but
+  // (with P in one part) 82.6 / 78.7 for 128 windows, 192 / 186 for 64 windows
+  // over 4000 tokens. Between 512 and 1024 pairs nothing was measured.
   const int64_t pairs = (int64_t)num_seqs * num_kv_heads;
   const int64_t pages = ((int64_t)max_context_len + block_size - 1) / block_size;
   int64_t per_pair = 3 * 148 / pairs;

@@ -34,10 +34,10 @@
 // with the join (6.3 TB/s; 291 us without any scores). mma.sync suffices: at 2
 // to 10 rows a 128-row tcgen05 tile would be empty. One sequence of 16381
 // tokens (68 MB) takes 17 us (3.9 TB/s; the split alone 13.4). fp8 pages and
-// windows are bound by instructions and by how evenly the contexts fall on the
-// SMs: 64 sequences of 200 to 1500 tokens take 30 us from fp8 pages (99 MB;
-// SMs busy 68% of the time, the schedulers issue in 42% of the cycles) and 48
-// us for windows of 5 f16 rows (197 MB).
+// windows are bound by how evenly the contexts fall on the SMs and by the chain
+// from MMA to softmax to MMA: 64 sequences of 200 to 1500 tokens take 31 us from
+// fp8 pages (99 MB; SMs busy 72% of the time, issuing in 45% of those cycles) and
+// 51 us for windows of 5 f16 rows (197 MB; 79% and 39%).
 #pragma once
 
 #include "decode_mma.cuh"
